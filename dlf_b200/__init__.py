@@ -94,6 +94,26 @@ def _declare(L):
     for fn in (L.dlf_b200_trmm, L.dlf_b200_trsm):
         fn.restype = c_int
         fn.argtypes = [c_int] * 6 + [c_size, c_size, c_void, c_void, c_size, c_void, c_size, c_void, c_size, c_void]
+    L.dlf_b200_quantize_rows.restype = c_int
+    L.dlf_b200_quantize_rows.argtypes = [c_int, c_size, c_size, c_void, c_size, c_void, c_size, c_void, c_void]
+    L.dlf_b200_gemm_int8.restype = c_int
+    L.dlf_b200_gemm_int8.argtypes = [c_int] + [c_size] * 3 + [c_void, c_size, c_void, c_void, c_size, c_void, c_void, c_int,
+                                                              c_void, c_size, c_void, c_size, c_void]
+    L.dlf_b200_gemm_int8_workspace_bytes.restype = c_size
+    L.dlf_b200_gemm_int8_workspace_bytes.argtypes = [c_size] * 3 + [c_void, c_size, c_void, c_size]
+    L.dlf_b200_attention_workspace_bytes.restype = c_size
+    L.dlf_b200_attention_workspace_bytes.argtypes = [c_size] * 6
+    L.dlf_b200_attention.restype = c_int
+    L.dlf_b200_attention.argtypes = [c_int] + [c_size] * 6 + [ctypes.c_float, c_void, c_void, c_void, c_void, c_void, c_void, c_void,
+                                                              c_void, c_size, c_void, c_void, c_void, c_size, c_void]
+    L.dlf_b200_paged_attention_workspace_bytes.restype = c_size
+    L.dlf_b200_paged_attention_workspace_bytes.argtypes = [c_size] * 4
+    L.dlf_b200_paged_attention.restype = c_int
+    L.dlf_b200_paged_attention.argtypes = [c_int] + [c_size] * 4 + [ctypes.c_float] + [c_void] * 6 + [
+        c_size, c_size, c_void, c_size, c_size, c_void, c_void, c_void, c_void, c_size, c_void]
+    L.dlf_b200_paged_append.restype = c_int
+    L.dlf_b200_paged_append.argtypes = [c_int] + [c_size] * 3 + [c_void] * 8 + [c_size, c_size, c_void, c_size, c_size, c_size,
+                                                                              c_void, c_void, c_void]
     L.dlf_b200_status_string.restype = ctypes.c_char_p
     L.dlf_b200_status_string.argtypes = [c_int]
     L.dlf_b200_device_status.restype = c_int
@@ -126,6 +146,14 @@ EXPORTED_SYMBOLS = (
     "dlf_b200_syrk",
     "dlf_b200_trmm",
     "dlf_b200_trsm",
+    "dlf_b200_quantize_rows",
+    "dlf_b200_gemm_int8",
+    "dlf_b200_gemm_int8_workspace_bytes",
+    "dlf_b200_attention_workspace_bytes",
+    "dlf_b200_attention",
+    "dlf_b200_paged_attention_workspace_bytes",
+    "dlf_b200_paged_attention",
+    "dlf_b200_paged_append",
     "dlf_b200_maxpool",
     "dlf_b200_avgpool",
     "dlf_b200_status_string",

@@ -27,6 +27,7 @@
 #include "contraction_split.cuh"
 #include "conv_small.cuh"
 #include "conv_halo.cuh"
+#include "host.cuh"
 #include "level3.cuh"
 #include "pooling.cuh"
 
@@ -34,26 +35,6 @@ using namespace dlfb200;
 
 namespace {
 
-// gpgpu::blas::StatusCode values used here (gpgpu/include/gblas.h:43-107)
-enum : int {
-    kSuccess = 0,
-    kInvalidValue = -30,
-    kNotImplemented = -1024,
-    kInvalidMatrixA = -1022,
-    kInvalidMatrixB = -1021,
-    kInvalidMatrixC = -1020,
-    kInvalidDimension = -1017,
-    kInvalidLeadDimA = -1016,
-    kInvalidLeadDimB = -1015,
-    kInvalidLeadDimC = -1014,
-    kInsufficientMemoryTemp = -2050,
-    kInvalidBatchCount = -2049,
-    kNoHalfPrecision = -2045,
-    kUnexpectedError = -2039,
-};
-
-constexpr int kMaxDevices = 64;
-constexpr int kSmemPerBlockOptin = 232448;  // 227 KB
 constexpr int kB200Sms = 148;  // for sizes that are asked for without a device at hand
 
 struct DeviceState {
@@ -85,60 +66,6 @@ std::mutex g_mu;
 std::atomic<unsigned long long> g_launches{0};
 std::atomic<int> g_force_bn{0};
 std::atomic<int> g_force_generic{0};
-
-#define CUDA_TRY(expr)                                   \
-    do {                                                 \
-        cudaError_t e__ = (expr);                        \
-        if (e__ != cudaSuccess) return static_cast<int>(e__); \
-    } while (0)
-
-// The device a call works on is the one its stream belongs to (the reference binds a queue to its
-// context's device, gpgpu/src/gpgpu_cu.cpp:174-204), not whatever device happens to be current on
-// the calling thread. The guard makes that device current for the duration of the call and puts
-// the previous one back; the legacy default stream (null) means the current device.
-struct StreamDevice {
-    int dev = 0;
-    int prev = -1;
-    int rc = kSuccess;
-    explicit StreamDevice(cudaStream_t s) {
-        cudaError_t e = cudaGetDevice(&dev);
-        if (e != cudaSuccess) {
-            rc = static_cast<int>(e);
-            return;
-        }
-        if (s != nullptr && s != cudaStreamLegacy && s != cudaStreamPerThread) {
-            // a stream that is being captured into a CUDA graph may not be queried (the query fails and
-            // invalidates the capture): such a call works on the current device, which a capture
-            // requires to be the stream's anyway
-            cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-            if (cudaStreamIsCapturing(s, &cap) != cudaSuccess) {
-                (void)cudaGetLastError();
-                cap = cudaStreamCaptureStatusNone;
-            }
-            if (cap != cudaStreamCaptureStatusNone) return;
-            int sd = dev;
-            e = cudaStreamGetDevice(s, &sd);
-            if (e != cudaSuccess) {
-                rc = static_cast<int>(e);
-                return;
-            }
-            if (sd != dev) {
-                e = cudaSetDevice(sd);
-                if (e != cudaSuccess) {
-                    rc = static_cast<int>(e);
-                    return;
-                }
-                prev = dev;
-                dev = sd;
-            }
-        }
-    }
-    ~StreamDevice() {
-        if (prev >= 0) (void)cudaSetDevice(prev);
-    }
-    StreamDevice(const StreamDevice&) = delete;
-    StreamDevice& operator=(const StreamDevice&) = delete;
-};
 
 // The tensor-memory-operand kernel exists once per element size and operand kind (see
 // contraction_ts.cuh): attributes are set on all of them, the largest static shared-memory use is
@@ -647,11 +574,6 @@ void set_wait_policy(Params& p, long long total_tiles) {
     p.skip_tile_commit = inject ? 1 : 0;
 }
 
-// A launch below is checked with cudaGetLastError(), which also returns an error that an earlier,
-// unrelated runtime call of this host thread left behind (non-sticky errors stay until read).
-// Such a leftover is not this call's failure: it is read away before the first launch.
-inline void clear_stale_error() { (void)cudaGetLastError(); }
-
 int launch_ts(const DeviceState& st, const Problem& q, cudaStream_t stream) {
     clear_stale_error();
     const int a_cols = q.es == 4 ? 64 : 32;
@@ -859,22 +781,6 @@ int launch_ts(const DeviceState& st, const Problem& q, cudaStream_t stream) {
     g_launches.fetch_add(1);
     CUDA_TRY(cudaGetLastError());
     return kSuccess;
-}
-
-// launch of a programmatic dependent of the kernel before it in the stream
-template <typename... Formal, typename... Actual>
-cudaError_t launch_dependent(void (*kernel)(Formal...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, Actual... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid, 1, 1);
-    cfg.blockDim = dim3(block, 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
 }
 
 // Whether a problem can go to contraction_f32_kernel: both operands through tensor maps, one alpha and beta, plain
@@ -1865,6 +1771,21 @@ int split_bank(Problem& q, const DeviceState& st, char* ws, const char* ws_end, 
 }
 
 }  // namespace
+
+namespace dlfb200 {
+int operator_device(OperatorDevice* out) {
+    DeviceState* st = nullptr;
+    const int rc = ensure_device(&st);
+    if (rc != kSuccess) return rc;
+    CUDA_TRY(cudaGetDevice(&out->device));
+    out->num_sms = st->num_sms;
+    out->status = st->status;
+    out->encode = st->encode;
+    return kSuccess;
+}
+unsigned tuning_bits() { return static_cast<unsigned>(g_force_generic.load()); }
+void count_launch() { g_launches.fetch_add(1); }
+}  // namespace dlfb200
 
 extern "C" {
 

@@ -1,0 +1,334 @@
+// extern "C" entries of attention (declared in include/dlf_b200.h): argument checks, the choice of the kernel, tensor maps
+// and launches.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "../../include/dlf_b200.h"
+#include "attention_decode.cuh"
+#include "attention_plan.h"
+#include "attention_tiles.cuh"
+#include "host.cuh"
+
+using namespace dlfb200;
+
+namespace {
+
+constexpr int kDecodeCtasPerSm = 2;
+constexpr int kDecodeLeast = 2;    // units a CTA takes at least
+constexpr long long kB200Sms = 148;  // for sizes that are asked for without a device at hand
+
+struct AttentionDevice {
+    bool ready = false;
+};
+AttentionDevice g_attention[kMaxDevices];
+std::mutex g_attention_mu;
+
+template <bool BF16, int DP>
+int attention_limits() {
+    CUDA_TRY(cudaFuncSetAttribute(attention_decode_kernel<BF16, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(DP)));
+    CUDA_TRY(cudaFuncSetAttribute(attention_decode_kernel<BF16, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(DP)));
+    CUDA_TRY(cudaFuncSetAttribute(attention_tiles_kernel<BF16, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, tiles_smem(DP)));
+    return kSuccess;
+}
+
+int attention_device(const OperatorDevice& dev) {
+    std::lock_guard<std::mutex> lock(g_attention_mu);
+    AttentionDevice& st = g_attention[dev.device];
+    if (st.ready) return kSuccess;
+    for (int rc : {attention_limits<false, 64>(), attention_limits<false, 128>(), attention_limits<true, 64>(), attention_limits<true, 128>()})
+        if (rc != kSuccess) return rc;
+    st.ready = true;
+    return kSuccess;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// strides that 16-byte pieces and tensor maps take
+bool strides_ok(std::initializer_list<size_t> s) {
+    for (size_t x : s)
+        if (x % 8 != 0 || x >= (1ull << 38)) return false;
+    return true;
+}
+
+size_t decode_workspace(int ctas, size_t size) { return static_cast<size_t>(2 * ctas) * decode_slot(static_cast<int>(size)) * 4; }
+
+template <bool BF16, int DP, bool PAGED>
+int decode_launch(const DecodeParams& p, cudaStream_t stream) {
+    CUDA_TRY(launch_dependent(attention_decode_kernel<BF16, DP, PAGED>, static_cast<unsigned>(p.ctas), kDecodeThreads, decode_smem(DP), stream, p));
+    count_launch();
+    CUDA_TRY(launch_dependent(attention_join_kernel<BF16>, static_cast<unsigned>(p.batch * p.kv_heads * p.row_blocks), 128u, 0, stream, p));
+    count_launch();
+    CUDA_TRY(cudaGetLastError());
+    return kSuccess;
+}
+int decode_any(const DecodeParams& p, bool bf16, bool paged, cudaStream_t stream) {
+    if (p.size <= 64) {
+        if (bf16) return paged ? decode_launch<true, 64, true>(p, stream) : decode_launch<true, 64, false>(p, stream);
+        return paged ? decode_launch<false, 64, true>(p, stream) : decode_launch<false, 64, false>(p, stream);
+    }
+    if (bf16) return paged ? decode_launch<true, 128, true>(p, stream) : decode_launch<true, 128, false>(p, stream);
+    return paged ? decode_launch<false, 128, true>(p, stream) : decode_launch<false, 128, false>(p, stream);
+}
+
+// tensor map of a (batch, tokens, heads, size) tensor: boxes of `rows` tokens x 64 values of one head, 128-byte swizzle
+int encode_heads(const OperatorDevice& dev, CUtensorMap* map, const void* base, size_t size, size_t tokens, size_t heads, size_t batch,
+                 size_t st, size_t sh, size_t sb, unsigned rows) {
+    auto stride = [](size_t extent, size_t s) { return static_cast<cuuint64_t>(extent > 1 && s > 0 ? s * 2 : 16); };
+    cuuint64_t dims[4] = {size, tokens, heads, sb == 0 ? 1 : batch};
+    cuuint64_t strides[3] = {stride(tokens, st), stride(heads, sh), stride(dims[3], sb)};
+    cuuint32_t box[4] = {64, rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+    const CUresult r = dev.encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? kSuccess : kUnexpectedError;
+}
+
+template <bool BF16, int DP>
+int tiles_launch(const TilesParams& p, unsigned grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& y,
+                 cudaStream_t stream) {
+    CUDA_TRY(launch_dependent(attention_tiles_kernel<BF16, DP>, grid, kTilesThreads, tiles_smem(DP), stream, p, q, k, v, y));
+    count_launch();
+    CUDA_TRY(cudaGetLastError());
+    return kSuccess;
+}
+
+// few query rows for each kv head: the kernel that reads the keys once for 16 rows
+bool few_rows(size_t queries, size_t group) { return queries * group <= 16; }
+
+int head_args(int dtype, size_t heads, size_t kv_heads, size_t size) {
+    if (dtype != DLF_B200_HALF && dtype != DLF_B200_BFLOAT16) return kNotImplemented;
+    if (heads == 0 || kv_heads == 0 || size == 0 || heads % kv_heads != 0 || heads > 65535) return kInvalidDimension;
+    if (size > 128 || size % 8 != 0) return kNotImplemented;
+    return kSuccess;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dlf_b200_attention_workspace_bytes(size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size) {
+    (void)batch;
+    (void)keys;
+    if (kv_heads == 0 || heads % kv_heads != 0) return 0;
+    return few_rows(queries, heads / kv_heads) ? decode_workspace(kDecodeCtasPerSm * kB200Sms, size) : 0;
+}
+
+int dlf_b200_attention(int dtype, size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size, float scale,
+                       const void* q, const size_t* q_strides, const void* k, const size_t* k_strides, const void* v,
+                       const size_t* v_strides, const int* key_lengths, const unsigned char* key_mask, size_t key_mask_ld, void* y,
+                       const size_t* y_strides, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = head_args(dtype, heads, kv_heads, size);
+    if (rc != kSuccess) return rc;
+    if (batch == 0 || queries == 0 || keys == 0 || batch > 65535 || queries > INT_MAX / 2 || keys > INT_MAX / 2) return kInvalidDimension;
+    if (!(scale > 0.0f) || std::isinf(scale)) return kInvalidValue;
+    if (q == nullptr || q_strides == nullptr) return kInvalidMatrixA;
+    if (k == nullptr || v == nullptr || k_strides == nullptr || v_strides == nullptr) return kInvalidMatrixB;
+    if (y == nullptr || y_strides == nullptr) return kInvalidMatrixC;
+    if (key_mask != nullptr && key_mask_ld < keys && batch > 1) return kInvalidLeadDimB;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(y) ||
+        !strides_ok({q_strides[0], q_strides[1], q_strides[2], k_strides[0], k_strides[1], k_strides[2], v_strides[0], v_strides[1], v_strides[2],
+                     y_strides[0], y_strides[1], y_strides[2]}))
+        return kNotImplemented;
+    if ((batch > 1 && y_strides[0] == 0) || (queries > 1 && y_strides[1] == 0) || (heads > 1 && y_strides[2] == 0)) return kInvalidLeadDimC;
+    if ((queries > 1 && q_strides[1] == 0) || (heads > 1 && q_strides[2] == 0)) return kInvalidLeadDimA;
+    if ((keys > 1 && (k_strides[1] == 0 || v_strides[1] == 0)) || (kv_heads > 1 && (k_strides[2] == 0 || v_strides[2] == 0))) return kInvalidLeadDimB;
+    const bool bf16 = dtype == DLF_B200_BFLOAT16;
+    const size_t group = heads / kv_heads;
+    const bool few = few_rows(queries, group);
+    if (few && (workspace == nullptr || workspace_bytes < dlf_b200_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, size)))
+        return kInsufficientMemoryTemp;
+    const long long items = static_cast<long long>((queries + 255) / 256) * static_cast<long long>(heads) * static_cast<long long>(batch);
+    if (items > INT_MAX / 2 || static_cast<double>(batch) * heads * (keys / kPlanUnit + 1.0) > 2147483647.0) return kInvalidDimension;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    StreamDevice guard(s);
+    if (guard.rc != kSuccess) return guard.rc;
+    OperatorDevice dev;
+    rc = operator_device(&dev);
+    if (rc != kSuccess) return rc;
+    rc = attention_device(dev);
+    if (rc != kSuccess) return rc;
+    clear_stale_error();
+    const float c = scale * 1.44269504088896340736f;
+    if (few) {
+        DecodeParams p{};
+        p.q = static_cast<const char*>(q);
+        p.k = static_cast<const char*>(k);
+        p.v = static_cast<const char*>(v);
+        p.y = static_cast<char*>(y);
+        p.q_sb = q_strides[0], p.q_st = q_strides[1], p.q_sh = q_strides[2];
+        p.k_sb = k_strides[0], p.k_st = k_strides[1], p.k_sh = k_strides[2];
+        p.v_sb = v_strides[0], p.v_st = v_strides[1], p.v_sh = v_strides[2];
+        p.y_sb = y_strides[0], p.y_st = y_strides[1], p.y_sh = y_strides[2];
+        p.lengths = key_lengths;
+        p.mask = key_mask;
+        p.mask_sb = static_cast<long long>(key_mask_ld);
+        p.page_size = 1;
+        p.batch = static_cast<int>(batch);
+        p.tokens = static_cast<int>(queries);
+        p.kv_heads = static_cast<int>(kv_heads);
+        p.group = static_cast<int>(group);
+        p.size = static_cast<int>(size);
+        p.keys = static_cast<int>(keys);
+        p.row_blocks = static_cast<int>((queries * group + 15) / 16);
+        p.ctas = std::min(kDecodeCtasPerSm * dev.num_sms, static_cast<int>(kDecodeCtasPerSm * kB200Sms));
+        p.least = kDecodeLeast;
+        p.c = c;
+        p.parts = static_cast<float*>(workspace);
+        p.status = dev.status;
+        return decode_any(p, bf16, false, s);
+    }
+    TilesParams p{};
+    p.batch = static_cast<int>(batch);
+    p.queries = static_cast<int>(queries);
+    p.keys = static_cast<int>(keys);
+    p.heads = static_cast<int>(heads);
+    p.kv_heads = static_cast<int>(kv_heads);
+    p.group = static_cast<int>(group);
+    p.size = static_cast<int>(size);
+    p.lengths = key_lengths;
+    p.mask = key_mask;
+    p.mask_sb = static_cast<long long>(key_mask_ld);
+    p.q_pairs = static_cast<int>((queries + 255) / 256);
+    p.items = static_cast<int>(items);
+    p.q_batched = q_strides[0] != 0;
+    p.k_batched = k_strides[0] != 0;
+    p.v_batched = v_strides[0] != 0;
+    p.c = c;
+    p.status = dev.status;
+    const bool inject = (tuning_bits() & 0x10000000u) != 0 && p.items == 1;
+    p.wait_limit = inject ? (1ll << 21) : (1ll << 32);
+    p.withhold = inject ? 1 : 0;
+    CUtensorMap mq, mk, mv, my;
+    rc = encode_heads(dev, &mq, q, size, queries, heads, batch, q_strides[1], q_strides[2], q_strides[0], 128);
+    if (rc == kSuccess) rc = encode_heads(dev, &mk, k, size, keys, kv_heads, batch, k_strides[1], k_strides[2], k_strides[0], 128);
+    if (rc == kSuccess) rc = encode_heads(dev, &mv, v, size, keys, kv_heads, batch, v_strides[1], v_strides[2], v_strides[0], 128);
+    if (rc == kSuccess) rc = encode_heads(dev, &my, y, size, queries, heads, batch, y_strides[1], y_strides[2], y_strides[0], 32);
+    if (rc != kSuccess) return rc;
+    const unsigned grid = static_cast<unsigned>(std::min<long long>(items, dev.num_sms));
+    if (size <= 64) return bf16 ? tiles_launch<true, 64>(p, grid, mq, mk, mv, my, s) : tiles_launch<false, 64>(p, grid, mq, mk, mv, my, s);
+    return bf16 ? tiles_launch<true, 128>(p, grid, mq, mk, mv, my, s) : tiles_launch<false, 128>(p, grid, mq, mk, mv, my, s);
+}
+
+size_t dlf_b200_paged_attention_workspace_bytes(size_t batch, size_t heads, size_t kv_heads, size_t size) {
+    (void)batch;
+    (void)heads;
+    (void)kv_heads;
+    return decode_workspace(kDecodeCtasPerSm * kB200Sms, size);
+}
+
+int dlf_b200_paged_attention(int dtype, size_t batch, size_t heads, size_t kv_heads, size_t size, float scale, const void* q,
+                             const size_t* q_strides, const void* k_pages, const size_t* k_strides, const void* v_pages,
+                             const size_t* v_strides, size_t num_pages, size_t page_size, const int* page_table, size_t table_width,
+                             size_t table_ld, const int* lengths, void* y, const size_t* y_strides, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+    int rc = head_args(dtype, heads, kv_heads, size);
+    if (rc != kSuccess) return rc;
+    if (batch == 0 || num_pages == 0 || page_size == 0 || table_width == 0 || batch > 65535 || num_pages > INT_MAX || page_size > INT_MAX ||
+        static_cast<double>(table_width) * static_cast<double>(page_size) > INT_MAX / 2)
+        return kInvalidDimension;
+    if (!(scale > 0.0f) || std::isinf(scale)) return kInvalidValue;
+    if (q == nullptr || q_strides == nullptr) return kInvalidMatrixA;
+    if (k_pages == nullptr || v_pages == nullptr || k_strides == nullptr || v_strides == nullptr || page_table == nullptr || lengths == nullptr)
+        return kInvalidMatrixB;
+    if (y == nullptr || y_strides == nullptr) return kInvalidMatrixC;
+    if (table_ld < table_width && batch > 1) return kInvalidLeadDimB;
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(y) ||
+        !strides_ok({q_strides[0], q_strides[1], k_strides[0], k_strides[1], k_strides[2], v_strides[0], v_strides[1], v_strides[2], y_strides[0],
+                     y_strides[1]}))
+        return kNotImplemented;
+    if ((batch > 1 && y_strides[0] == 0) || (heads > 1 && y_strides[1] == 0)) return kInvalidLeadDimC;
+    if (static_cast<double>(batch) * heads * (static_cast<double>(table_width) * page_size / kPlanUnit + 1.0) > 2147483647.0) return kInvalidDimension;
+    if (workspace == nullptr || workspace_bytes < dlf_b200_paged_attention_workspace_bytes(batch, heads, kv_heads, size)) return kInsufficientMemoryTemp;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    StreamDevice guard(s);
+    if (guard.rc != kSuccess) return guard.rc;
+    OperatorDevice dev;
+    rc = operator_device(&dev);
+    if (rc != kSuccess) return rc;
+    rc = attention_device(dev);
+    if (rc != kSuccess) return rc;
+    clear_stale_error();
+    DecodeParams p{};
+    p.q = static_cast<const char*>(q);
+    p.k = static_cast<const char*>(k_pages);
+    p.v = static_cast<const char*>(v_pages);
+    p.y = static_cast<char*>(y);
+    p.q_sb = q_strides[0], p.q_sh = q_strides[1];
+    p.k_sb = k_strides[0], p.k_st = k_strides[1], p.k_sh = k_strides[2];
+    p.v_sb = v_strides[0], p.v_st = v_strides[1], p.v_sh = v_strides[2];
+    p.y_sb = y_strides[0], p.y_sh = y_strides[1];
+    p.lengths = lengths;
+    p.table = page_table;
+    p.table_sb = static_cast<long long>(table_ld);
+    p.page_size = static_cast<int>(page_size);
+    p.num_pages = static_cast<int>(num_pages);
+    p.batch = static_cast<int>(batch);
+    p.tokens = 1;
+    p.kv_heads = static_cast<int>(kv_heads);
+    p.group = static_cast<int>(heads / kv_heads);
+    p.size = static_cast<int>(size);
+    p.keys = static_cast<int>(table_width * page_size);
+    p.row_blocks = (p.group + 15) / 16;
+    p.ctas = std::min(kDecodeCtasPerSm * dev.num_sms, static_cast<int>(kDecodeCtasPerSm * kB200Sms));
+    p.least = kDecodeLeast;
+    p.c = scale * 1.44269504088896340736f;
+    p.parts = static_cast<float*>(workspace);
+    p.status = dev.status;
+    return decode_any(p, dtype == DLF_B200_BFLOAT16, true, s);
+}
+
+int dlf_b200_paged_append(int dtype, size_t tokens, size_t kv_heads, size_t size, const void* k, const size_t* k_strides, const void* v,
+                          const size_t* v_strides, void* k_pages, const size_t* kp_strides, void* v_pages, const size_t* vp_strides,
+                          size_t num_pages, size_t page_size, const int* page_table, size_t batch, size_t table_width, size_t table_ld,
+                          const int* positions, const int* sequences, void* stream) {
+    int rc = head_args(dtype, kv_heads, kv_heads, size);
+    if (rc != kSuccess) return rc;
+    if (tokens == 0 || batch == 0 || num_pages == 0 || page_size == 0 || table_width == 0 || tokens > INT_MAX || batch > INT_MAX || num_pages > INT_MAX ||
+        page_size > INT_MAX || table_width > INT_MAX || kv_heads * size > INT_MAX)
+        return kInvalidDimension;
+    if (sequences == nullptr && tokens > batch) return kInvalidDimension;
+    if (k == nullptr || v == nullptr || k_strides == nullptr || v_strides == nullptr) return kInvalidMatrixA;
+    if (page_table == nullptr || positions == nullptr) return kInvalidMatrixB;
+    if (k_pages == nullptr || v_pages == nullptr || kp_strides == nullptr || vp_strides == nullptr) return kInvalidMatrixC;
+    if (table_ld < table_width && batch > 1) return kInvalidLeadDimB;
+    if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) ||
+        !strides_ok({k_strides[0], k_strides[1], v_strides[0], v_strides[1], kp_strides[0], kp_strides[1], kp_strides[2], vp_strides[0], vp_strides[1],
+                     vp_strides[2]}))
+        return kNotImplemented;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    StreamDevice guard(s);
+    if (guard.rc != kSuccess) return guard.rc;
+    OperatorDevice dev;
+    rc = operator_device(&dev);
+    if (rc != kSuccess) return rc;
+    clear_stale_error();
+    AppendParams p{};
+    p.k = static_cast<const char*>(k);
+    p.v = static_cast<const char*>(v);
+    p.k_pages = static_cast<char*>(k_pages);
+    p.v_pages = static_cast<char*>(v_pages);
+    p.k_st = k_strides[0], p.k_sh = k_strides[1], p.v_st = v_strides[0], p.v_sh = v_strides[1];
+    p.kp_sb = kp_strides[0], p.kp_st = kp_strides[1], p.kp_sh = kp_strides[2];
+    p.vp_sb = vp_strides[0], p.vp_st = vp_strides[1], p.vp_sh = vp_strides[2];
+    p.table = page_table;
+    p.table_sb = static_cast<long long>(table_ld);
+    p.positions = positions;
+    p.sequences = sequences;
+    p.tokens = static_cast<int>(tokens);
+    p.batch = static_cast<int>(batch);
+    p.table_width = static_cast<int>(std::min<size_t>(table_width, INT_MAX / 2));
+    p.page_size = static_cast<int>(page_size);
+    p.num_pages = static_cast<int>(num_pages);
+    p.kv_heads = static_cast<int>(kv_heads);
+    p.size = static_cast<int>(size);
+    p.status = dev.status;
+    const long long total = static_cast<long long>(tokens) * static_cast<long long>(kv_heads) * (static_cast<long long>(size) / 8);
+    CUDA_TRY(launch_dependent(paged_append_kernel, static_cast<unsigned>(std::min<long long>((total + 255) / 256, 16ll * dev.num_sms)), 256u, 0, s, p));
+    count_launch();
+    CUDA_TRY(cudaGetLastError());
+    return kSuccess;
+}
+
+}  // extern "C"

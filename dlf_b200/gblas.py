@@ -327,6 +327,114 @@ def _gemm(layout, a_transpose, b_transpose, m, n, k, alpha, a, a_ld, b, b_ld, be
     _check(rc)
 
 
+# ---------------------------------------------------------------------------------------------
+# Products in 8-bit integers. The reference has no such routine; names and argument order follow gemm.
+
+_INT8_WORKSPACES = {}
+
+
+def _operator_stream(queue, device):
+    """The raw stream of a call whose tensors lie on `device`; a stream of another device is refused."""
+    if queue is not None:
+        index, handle = queue.device_index, queue.cuda_stream
+    else:
+        index = torch._C._cuda_getDevice()
+        handle = torch._C._cuda_getCurrentRawStream(index)
+    if device.index != index:
+        raise BLASError(StatusCode.kInvalidValue)
+    return handle
+
+
+def _operator_scratch(table, need, device, queue, handle):
+    """(buffer, entry) for a call that cannot do without `need` bytes: the caller's buffer, one from the graph's pool or too
+    large to be kept, or (with entry) the stream's, to be asked for with the entry's lock held."""
+    ws = _caller_scratch(device, need)
+    if ws is not None:
+        return ws, None
+    with torch.cuda.stream(queue) if queue is not None else _NO_LOCK:
+        passing = need > _KEPT_BYTES or _capturing()
+    if passing:
+        ws = _passing_scratch(need, device, queue)
+        if ws is None:
+            raise BLASError(StatusCode.kInsufficientMemoryTemp)
+        return ws, None
+    return None, _stream_scratch(table, device, handle)
+
+
+def quantizeRows(m, n, x_buffer, x_offset, x_ld, q_buffer, q_offset, q_ld, scales, queue=None, event=None):
+    """Row i of X (m x n) to 8-bit integers in Q and the scale in scales[i] that they are to be multiplied with:
+    scales[i] = max |X[i]| / 127 and Q[i] = X[i] / scales[i], rounded to the nearest whole number (ties to even). A row that
+    holds an infinity or a NaN gets the scale NaN and zeros."""
+    _quantize_rows(m, n, _buffer_operand(x_buffer, x_offset), x_ld, _buffer_operand(q_buffer, q_offset), q_ld, scales, queue, event)
+
+
+def _quantize_rows(m, n, x, x_ld, q, q_ld, scales, queue=None, event=None):
+    prec = precision_of(x)
+    if q.dtype != torch.int8 or scales.dtype != torch.float32:
+        raise BLASError(StatusCode.kInvalidValue)
+    if m == 0 or n == 0:
+        raise BLASError(StatusCode.kInvalidDimension)
+    _test_matrix(n, m, x, x.offset, x_ld, StatusCode.kInvalidLeadDimA, StatusCode.kInsufficientMemoryA)
+    _test_matrix(n, m, q, q.offset, q_ld, StatusCode.kInvalidLeadDimC, StatusCode.kInsufficientMemoryC)
+    if scales.numel() < m or not scales.is_contiguous():
+        raise BLASError(StatusCode.kInsufficientMemoryC)
+    if not (x.is_cuda and x.device == q.device == scales.device):
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    handle = _operator_stream(queue, x.device)
+    if event is not None:
+        s = queue if queue is not None else torch.cuda.current_stream()
+        event.start.record(s)
+    rc = lib().dlf_b200_quantize_rows(int(prec), m, n, x.address, x_ld, q.address, q_ld, scales.data_ptr(), handle)
+    if event is not None:
+        event.end.record(s)
+    _check(rc)
+
+
+def gemmInt8(m, n, k, a_buffer, a_offset, a_ld, a_scales, b_buffer, b_offset, b_ld, b_scales, c_buffer, c_offset, c_ld, bias=None,
+             activation=None, queue=None, event=None):
+    """C[i][j] = act((sum_k A[i][k] * B[j][k]) * b_scales[j] * a_scales[i] + bias[j]): A (m x k) and B (n x k) 8-bit
+    integers, row-major, a scale for each of their rows; C (m x n) float16, bfloat16 or float32. The sums are exact."""
+    _gemm_int8(m, n, k, _buffer_operand(a_buffer, a_offset), a_ld, a_scales, _buffer_operand(b_buffer, b_offset), b_ld, b_scales,
+               _buffer_operand(c_buffer, c_offset), c_ld, bias, activation, queue, event)
+
+
+def _gemm_int8(m, n, k, a, a_ld, a_scales, b, b_ld, b_scales, c, c_ld, bias=None, activation=None, queue=None, event=None):
+    prec = precision_of(c)
+    if (a.dtype != torch.int8 or b.dtype != torch.int8 or a_scales.dtype != torch.float32 or b_scales.dtype != torch.float32 or
+            (bias is not None and bias.dtype != c.dtype) or activation not in (None, "relu")):
+        raise BLASError(StatusCode.kInvalidValue)
+    if m == 0 or n == 0 or k == 0:
+        raise BLASError(StatusCode.kInvalidDimension)
+    _test_matrix(k, m, a, a.offset, a_ld, StatusCode.kInvalidLeadDimA, StatusCode.kInsufficientMemoryA)
+    _test_matrix(k, n, b, b.offset, b_ld, StatusCode.kInvalidLeadDimB, StatusCode.kInsufficientMemoryB)
+    _test_matrix(n, m, c, c.offset, c_ld, StatusCode.kInvalidLeadDimC, StatusCode.kInsufficientMemoryC)
+    if a_scales.numel() < m or not a_scales.is_contiguous():
+        raise BLASError(StatusCode.kInsufficientMemoryA)
+    if b_scales.numel() < n or not b_scales.is_contiguous():
+        raise BLASError(StatusCode.kInsufficientMemoryB)
+    if bias is not None and (bias.numel() < n or not bias.is_contiguous()):
+        raise BLASError(StatusCode.kInvalidValue)
+    device = c.device
+    if not c.is_cuda or any(t.device != device for t in (a, b, a_scales, b_scales)) or (bias is not None and bias.device != device):
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    L = lib()
+    handle = _operator_stream(queue, device)
+    need = L.dlf_b200_gemm_int8_workspace_bytes(m, n, k, a.address, a_ld, b.address, b_ld)
+    ws, entry = _operator_scratch(_INT8_WORKSPACES, need, device, queue, handle) if need else (None, None)
+    with entry.lock if entry is not None else _NO_LOCK:
+        if entry is not None:
+            ws = entry.at_least(need, device, queue)
+        if event is not None:
+            s = queue if queue is not None else torch.cuda.current_stream()
+            event.start.record(s)
+        rc = L.dlf_b200_gemm_int8(int(prec), m, n, k, a.address, a_ld, a_scales.data_ptr(), b.address, b_ld, b_scales.data_ptr(),
+                                  bias.data_ptr() if bias is not None else None, 1 if activation == "relu" else 0, c.address, c_ld,
+                                  ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, handle)
+        if event is not None:
+            event.end.record(s)
+    _check(rc)
+
+
 def gemmStridedBatched(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_offset, a_ld,
                        a_stride, b_buffer, b_offset, b_ld, b_stride, beta, c_buffer, c_offset,
                        c_ld, c_stride, batch_count, queue=None, event=None):

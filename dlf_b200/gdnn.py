@@ -7,12 +7,13 @@
 convolution's epilogue.
 """
 import ctypes
+import math
 
 import torch
 
 from . import lib
-from .gblas import (BLASError, StatusCode, _NO_LOCK, _caller_scratch, _capturing, _check, _passing_scratch, _ptr, _stream,
-                    _stream_scratch, precision_of)
+from .gblas import (BLASError, StatusCode, _NO_LOCK, _caller_scratch, _capturing, _check, _operator_scratch, _operator_stream,
+                    _passing_scratch, _ptr, _stream, _stream_scratch, precision_of)
 
 
 class Filter2D:
@@ -312,3 +313,154 @@ def pool_nhwc(X, Y, filt, average=False, count_include_pad=False, queue=None):
     _check(lib().dlf_b200_pool_nhwc(int(prec), 1 if average else 0, 1 if count_include_pad else 0, f.batches, f.channels,
                                     f.height, f.width, f.output_h, f.output_w, f.kernel_h, f.kernel_w, f.pad_top,
                                     f.pad_left, f.stride_h, f.stride_w, _ptr(X), _ptr(Y), sp))
+
+
+# ---------------------------------------------------------------------------------------------
+# Attention over an encoder's states and over a paged cache (16-bit). The reference leaves its parts to its users: two batched
+# products and a softmax between them.
+
+_ATTENTION_WORKSPACES = {}
+_THREE = ctypes.c_size_t * 3
+_INT8_TYPES = (torch.bool, torch.uint8)
+
+
+def _head_tensor(t, dtype, device, dims):
+    """Checks a tensor of heads; its strides without the last dimension's."""
+    if t.dtype != dtype:
+        raise BLASError(StatusCode.kInvalidValue)
+    if t.dim() != dims:
+        raise BLASError(StatusCode.kInvalidDimension)
+    if t.device != device:
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    s = t.stride()
+    if s[-1] != 1 and t.shape[-1] != 1:
+        raise BLASError(StatusCode.kNotImplemented)
+    return s
+
+
+def _strides(shape, strides):
+    """Strides for the library; where there is only one, 8 elements stand for whatever is written."""
+    return _THREE(*[s if n > 1 else 8 for n, s in zip(shape[:-1], strides)])
+
+
+def _device_ints(t, count, device):
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise BLASError(StatusCode.kInvalidValue)
+    if t.numel() != count:
+        raise BLASError(StatusCode.kInvalidDimension)
+    if t.device != device:
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    return t.data_ptr()
+
+
+def _default_scale(scale, size):
+    scale = 1.0 / math.sqrt(size) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise BLASError(StatusCode.kInvalidValue)
+    return scale
+
+
+def _attention_call(need, device, queue, event, call):
+    """call(workspace, bytes, stream) with scratch of `need` bytes."""
+    handle = _operator_stream(queue, device)
+    ws, entry = _operator_scratch(_ATTENTION_WORKSPACES, need, device, queue, handle) if need else (None, None)
+    with entry.lock if entry is not None else _NO_LOCK:
+        if entry is not None:
+            ws = entry.at_least(need, device, queue)
+        if event is not None:
+            s = queue if queue is not None else torch.cuda.current_stream()
+            event.start.record(s)
+        rc = call(ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, handle)
+        if event is not None:
+            event.end.record(s)
+    _check(rc)
+
+
+def attention(Q, K, V, Y, scale=None, key_lengths=None, key_mask=None, queue=None, event=None):
+    """Y = softmax(scale * Q K^T) V for each head: the queries Q (batch, queries, heads, size) over the keys K and values V (batch,
+    keys, kv_heads, size) of another length, for instance an encoder's states. float16 or bfloat16, size a multiple of 8 up to
+    128, heads a multiple of kv_heads (head h reads kv head h // (heads // kv_heads)); ``scale`` is 1 / sqrt(size) if not given.
+
+    ``key_lengths`` (batch, int32) and ``key_mask`` (batch, keys; bool or uint8, 0 = left out) say which keys count; those that do not
+    may hold anything. A query with no key gets zeros. Any strides that are multiples of 8 elements, over 16-byte aligned
+    addresses, with a head's values contiguous; K and V may be shared by the batch (expanded)."""
+    device, dtype = Y.device, Y.dtype
+    prec = precision_of(Y)
+    qs, ks, vs, ys = (_head_tensor(t, dtype, device, 4) for t in (Q, K, V, Y))
+    b, lq, h, d = Q.shape
+    lk, hk = K.shape[1:3]
+    if K.shape[0] != b or K.shape[3] != d or V.shape != K.shape or Y.shape != Q.shape or 0 in Q.shape or 0 in K.shape or h % hk:
+        raise BLASError(StatusCode.kInvalidDimension)
+    scale = _default_scale(scale, d)
+    lengths = _device_ints(key_lengths, b, device) if key_lengths is not None else None
+    mask, mask_ld = None, 0
+    if key_mask is not None:
+        if key_mask.dtype not in _INT8_TYPES or tuple(key_mask.shape) != (b, lk) or (lk > 1 and key_mask.stride(1) != 1):
+            raise BLASError(StatusCode.kInvalidValue)
+        if key_mask.device != device:
+            raise BLASError(StatusCode.kInvalidMatrixA)
+        mask, mask_ld = key_mask.data_ptr(), key_mask.stride(0) if b > 1 else lk
+    if not Y.is_cuda:
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    L = lib()
+    _attention_call(L.dlf_b200_attention_workspace_bytes(b, lq, lk, h, hk, d), device, queue, event,
+                    lambda ws, n, stream: L.dlf_b200_attention(
+                        int(prec), b, lq, lk, h, hk, d, scale, Q.data_ptr(), _strides(Q.shape, qs), K.data_ptr(), _strides(K.shape, ks),
+                        V.data_ptr(), _strides(V.shape, vs), lengths, mask, mask_ld, Y.data_ptr(), _strides(Y.shape, ys), ws, n, stream))
+
+
+def _cache_tensors(K_pages, V_pages, page_table, dtype, device):
+    ks, vs = (_head_tensor(t, dtype, device, 4) for t in (K_pages, V_pages))
+    if V_pages.shape != K_pages.shape or 0 in K_pages.shape or page_table.dim() != 2 or 0 in page_table.shape:
+        raise BLASError(StatusCode.kInvalidDimension)
+    if page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise BLASError(StatusCode.kInvalidValue)
+    if page_table.device != device:
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    width = page_table.shape[1]
+    return _strides(K_pages.shape, ks), _strides(V_pages.shape, vs), width, page_table.stride(0) if page_table.shape[0] > 1 else width
+
+
+def paged_attention(Q, K_pages, V_pages, page_table, lengths, Y, scale=None, queue=None, event=None):
+    """Attention of one new token of every sequence over its paged cache: Q and Y (batch, heads, size), the cache K_pages and
+    V_pages (pages, page_size, kv_heads, size; any strides as in ``attention``). Position i of sequence b lies in page
+    page_table[b][i // page_size] (int32) at i % page_size; lengths[b] (int32) positions count, the new token's among them if
+    ``paged_append`` has put it there. Table entries beyond a sequence's length may be anything."""
+    device, dtype = Y.device, Y.dtype
+    prec = precision_of(Y)
+    qs, ys = _head_tensor(Q, dtype, device, 3), _head_tensor(Y, dtype, device, 3)
+    b, h, d = Q.shape
+    kst, vst, width, ld = _cache_tensors(K_pages, V_pages, page_table, dtype, device)
+    pages, page_size, hk, dk = K_pages.shape
+    if dk != d or Y.shape != Q.shape or 0 in Q.shape or page_table.shape[0] != b or h % hk:
+        raise BLASError(StatusCode.kInvalidDimension)
+    scale = _default_scale(scale, d)
+    n = _device_ints(lengths, b, device)
+    if not Y.is_cuda:
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    L = lib()
+    _attention_call(L.dlf_b200_paged_attention_workspace_bytes(b, h, hk, d), device, queue, event,
+                    lambda ws, nbytes, stream: L.dlf_b200_paged_attention(
+                        int(prec), b, h, hk, d, scale, Q.data_ptr(), _strides(Q.shape, qs), K_pages.data_ptr(), kst, V_pages.data_ptr(), vst,
+                        pages, page_size, page_table.data_ptr(), width, ld, n, Y.data_ptr(), _strides(Y.shape, ys), ws, nbytes, stream))
+
+
+def paged_append(K, V, K_pages, V_pages, page_table, positions, sequences=None, queue=None, event=None):
+    """New keys and values K and V (tokens, kv_heads, size) into a paged cache (see ``paged_attention``): token i to position
+    positions[i] of sequence sequences[i] (both int32; without ``sequences``, of sequence i). The rest of the cache stays as it is."""
+    device, dtype = K_pages.device, K_pages.dtype
+    prec = precision_of(K_pages)
+    kns, vns = _head_tensor(K, dtype, device, 3), _head_tensor(V, dtype, device, 3)
+    kst, vst, width, ld = _cache_tensors(K_pages, V_pages, page_table, dtype, device)
+    pages, page_size, hk, d = K_pages.shape
+    t = K.shape[0]
+    if K.shape != V.shape or tuple(K.shape[1:]) != (hk, d) or t == 0 or (sequences is None and t > page_table.shape[0]):
+        raise BLASError(StatusCode.kInvalidDimension)
+    pos = _device_ints(positions, t, device)
+    seq = _device_ints(sequences, t, device) if sequences is not None else None
+    if not K_pages.is_cuda:
+        raise BLASError(StatusCode.kInvalidMatrixA)
+    _attention_call(0, device, queue, event,
+                    lambda ws, n, stream: lib().dlf_b200_paged_append(
+                        int(prec), t, hk, d, K.data_ptr(), _strides(K.shape, kns), V.data_ptr(), _strides(V.shape, vns), K_pages.data_ptr(), kst,
+                        V_pages.data_ptr(), vst, pages, page_size, page_table.data_ptr(), page_table.shape[0], width, ld, pos, seq, stream))

@@ -253,6 +253,68 @@ def matmul(A, B, C=None, alpha=1, beta=0, backend=None, trace=None):
     return C
 
 
+def _rows(t, what):
+    """A (..., n) tensor as a matrix of its rows: (matrix, rows, n, elements between rows)."""
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, t.shape[-1])
+        except RuntimeError:
+            raise ShapeError("%s: the rows must be evenly spaced" % what)
+    m, n = t.shape
+    ld, inc = t.stride()
+    if inc != 1 and n > 1:
+        raise ShapeError("%s: rows must be contiguous" % what)
+    return t, m, n, ld if m > 1 else max(ld, n)
+
+
+def quantize(X, Q=None, scales=None):
+    """The rows of X (..., n) as 8-bit integers Q (..., n) and fp32 scales (...): row = Q * scale, to within half a scale
+    (``gblas.quantizeRows``). Returns (Q, scales). A Q allocated here has rows on 16-byte boundaries, the form that
+    ``matmul_int8`` reads without a copy."""
+    if X.dim() < 1:
+        raise ShapeError("quantize: X must have rows")
+    if Q is None:
+        n = X.shape[-1]
+        Q = torch.empty(X.shape[:-1] + ((n + 15) // 16 * 16,), dtype=torch.int8, device=X.device)[..., :n]
+    elif Q.shape != X.shape:
+        raise ShapeError("quantize: Q must have the shape of X")
+    if scales is None:
+        scales = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
+    elif scales.shape != X.shape[:-1]:
+        raise ShapeError("quantize: one scale for each row of X")
+    if not scales.is_contiguous():
+        raise ShapeError("quantize: the scales must be contiguous")
+    x, m, n, x_ld = _rows(X, "quantize")
+    q, _, _, q_ld = _rows(Q, "quantize")
+    _gblas._quantize_rows(m, n, _gblas._view_operand(x), x_ld, _gblas._view_operand(q), q_ld, scales)
+    return Q, scales
+
+
+def matmul_int8(A, a_scales, B, b_scales, C=None, bias=None, activation=None, dtype=torch.float32):
+    """C = act((A @ B^T) * a_scales * b_scales + bias) for 8-bit integers A (..., k) with a scale for each row (token) and B (n, k)
+    with one for each of its rows (output channel): a quantised layer (``gblas.gemmInt8``). C (..., n) is allocated with
+    ``dtype`` when not given."""
+    if A.dim() < 1 or B.dim() != 2:
+        raise ShapeError("matmul_int8: A must have rows and B must be a matrix")
+    if A.shape[-1] != B.shape[1]:
+        raise ShapeError("matmul_int8: incompatible shape")
+    if a_scales.shape != A.shape[:-1] or tuple(b_scales.shape) != (B.shape[0],):
+        raise ShapeError("matmul_int8: one scale for each row of A and of B")
+    shape = A.shape[:-1] + (B.shape[0],)
+    if C is None:
+        C = torch.empty(shape, dtype=dtype, device=A.device)
+    elif C.shape != shape:
+        raise ShapeError("matmul_int8: bad output shape")
+    if bias is not None and tuple(bias.shape) != (B.shape[0],):
+        raise ShapeError("matmul_int8: one bias for each row of B")
+    a, m, k, a_ld = _rows(A, "matmul_int8")
+    b, n, _, b_ld = _rows(B, "matmul_int8")
+    c, _, _, c_ld = _rows(C, "matmul_int8")
+    v = _gblas._view_operand
+    _gblas._gemm_int8(m, n, k, v(a), a_ld, a_scales, v(b), b_ld, b_scales, v(c), c_ld, bias, activation)
+    return C
+
+
 def dot(A, B, backend=None):
     """dlf::dot (linalg.h:511-549): scalars scale, everything else is matmul after the N-D
     operand's contraction axis is brought to matmul's convention."""

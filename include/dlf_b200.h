@@ -246,6 +246,72 @@ int dlf_b200_avgpool(int dtype, size_t batches, size_t channels, size_t height, 
                      size_t stride_h, size_t stride_w, size_t dilation_h, size_t dilation_w,
                      int count_include_pad, const void* x, void* y, void* stream);
 
+/* Products in 8-bit integers with a scale for each row of A (token) and each row of B (output channel), the form of a
+ * quantised layer. No counterpart in the reference, whose gemm takes floating-point matrices.
+ *
+ * dlf_b200_quantize_rows: row i of X (rows x cols, storage type `dtype`) to integers and the scale that they are to be
+ * multiplied with:
+ *     scales[i] = max(max_j |X[i][j]| / 127, 2^-126)            (rounded to fp32 once)
+ *     Q[i][j]   = the whole number nearest to X[i][j] / scales[i], the even one of two equally near
+ * A row that holds an infinity or a NaN gets the scale NaN and zeros, so its products are NaN. X and Q may be padded
+ * (x_ld, q_ld >= cols); the padding is neither read nor written. X and Q must not overlap.
+ *
+ * dlf_b200_gemm_int8: C[i][j] = act((sum_k A[i][k] * B[j][k]) * b_scales[j] * a_scales[i] + bias[j]), A m x k, B n x k (both
+ * with their k values contiguous), C m x n of type `dtype`, row-major. The sums are exact 32-bit integers, hence
+ * k <= 131071 (kInvalidDimension beyond); they are scaled in fp32 and rounded to C's type once. `bias` (n values of C's
+ * type) may be NULL; `activation` as in dlf_b200_conv2d_fused. Operands whose lines are not 16-byte aligned (base and
+ * leading dimension) are copied into `workspace` first: dlf_b200_gemm_int8_workspace_bytes bytes of device memory, 0 for
+ * aligned operands; kInsufficientMemoryTemp, and nothing launched, if there is less. C must not overlap the operands. */
+int dlf_b200_quantize_rows(int dtype, size_t rows, size_t cols, const void* x, size_t x_ld, signed char* q, size_t q_ld,
+                           float* scales, void* stream);
+int dlf_b200_gemm_int8(int dtype, size_t m, size_t n, size_t k, const signed char* a, size_t a_ld, const float* a_scales,
+                       const signed char* b, size_t b_ld, const float* b_scales, const void* bias, int activation, void* c,
+                       size_t c_ld, void* workspace, size_t workspace_bytes, void* stream);
+size_t dlf_b200_gemm_int8_workspace_bytes(size_t m, size_t n, size_t k, const signed char* a, size_t a_ld, const signed char* b,
+                                          size_t b_ld);
+
+/* Attention of the queries of a decoder (or of an image) over an encoder's states, or of one new token over a paged cache:
+ *     Y = softmax(scale * Q K^T over the kept keys) V                    for each head
+ * with 32-bit scores, softmax statistics and sums. Types: Half and BFloat16 (else kNotImplemented). `heads` query heads share
+ * `kv_heads` heads of keys and values (heads a multiple of kv_heads; head h reads kv head h / (heads / kv_heads)). A head's
+ * `size` values are contiguous: a multiple of 8 up to 128. The other strides are counted in elements and arbitrary, but multiples
+ * of 8 over 16-byte aligned bases (kNotImplemented else). scale > 0. A row of which no key is kept is zeros. What is
+ * masked out is not used, whatever it is (infinities, NaN). Nothing is kept between calls.
+ *
+ * dlf_b200_attention: Q and Y are (batch, queries, heads, size) with strides {batch, token, head}, K and V (batch, keys,
+ * kv_heads, size) with theirs; a batch stride of 0 shares Q, K or V between the batch's entries. `key_lengths` (batch, device, or
+ * NULL): keys of each entry that count, the rest is padding. `key_mask` (batch, keys, bytes; lines key_mask_ld apart; device, or
+ * NULL): 0 = the key does not count. `workspace`: dlf_b200_attention_workspace_bytes bytes of device memory (0 where none is
+ * needed). Y must not overlap the inputs.
+ *
+ * dlf_b200_paged_attention: one query token for each sequence. Q and Y are (batch, heads, size) with strides {batch, head}; the
+ * cache is (num_pages, page_size, kv_heads, size) with strides {page, token, head}; position i of sequence b lies in page
+ * page_table[b][i / page_size] (device, int32, lines table_ld apart, table_width entries each) at i % page_size; lengths[b]
+ * (device) positions are kept.
+ *
+ * dlf_b200_paged_append: token i of K and V (tokens, kv_heads, size; strides {token, head}) to position positions[i] of
+ * sequence sequences[i] (both device, int32; sequences == NULL: sequence i). Where two tokens go to one position, either's
+ * values are found there.
+ *
+ * Lengths below 0 count as 0 and those beyond the keys there are as all of them; keys on a page that is none of the
+ * num_pages do not count, and tokens for a position or page that does not exist are left out. Such lengths, positions and pages are
+ * reported by bit 1 of dlf_b200_device_status (a length below 0 is not); nothing outside the tensors is read or written. */
+size_t dlf_b200_attention_workspace_bytes(size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size);
+int dlf_b200_attention(int dtype, size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size, float scale,
+                       const void* q, const size_t* q_strides, const void* k, const size_t* k_strides, const void* v,
+                       const size_t* v_strides, const int* key_lengths, const unsigned char* key_mask, size_t key_mask_ld, void* y,
+                       const size_t* y_strides, void* workspace, size_t workspace_bytes, void* stream);
+size_t dlf_b200_paged_attention_workspace_bytes(size_t batch, size_t heads, size_t kv_heads, size_t size);
+int dlf_b200_paged_attention(int dtype, size_t batch, size_t heads, size_t kv_heads, size_t size, float scale, const void* q,
+                             const size_t* q_strides, const void* k_pages, const size_t* k_strides, const void* v_pages,
+                             const size_t* v_strides, size_t num_pages, size_t page_size, const int* page_table, size_t table_width,
+                             size_t table_ld, const int* lengths, void* y, const size_t* y_strides, void* workspace,
+                             size_t workspace_bytes, void* stream);
+int dlf_b200_paged_append(int dtype, size_t tokens, size_t kv_heads, size_t size, const void* k, const size_t* k_strides, const void* v,
+                          const size_t* v_strides, void* k_pages, const size_t* kp_strides, void* v_pages, const size_t* vp_strides,
+                          size_t num_pages, size_t page_size, const int* page_table, size_t batch, size_t table_width,
+                          size_t table_ld, const int* positions, const int* sequences, void* stream);
+
 /* Name of a status code returned by the functions above (static storage). Mirrors the
  * StatusCode enumerators of gblas.h:43-107. */
 const char* dlf_b200_status_string(int status);
