@@ -11,7 +11,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libdlf_b200.so")
-OBJECTS = CSRC  # (*.o beside the sources)
+OBJECTS = os.path.join(HERE, "objects")
 SOURCES = ["api.cu", "quantized.cu", "attention.cu"]
 
 
@@ -62,6 +62,7 @@ def build(force=False, verbose=False):
     """Compile the CUDA sources (one process each) and link libdlf_b200.so; returns the library path."""
     if not force and not _stale():
         return LIB
+    os.makedirs(OBJECTS, exist_ok=True)
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     arch = ["-gencode", "arch=compute_100a,code=sm_100a"]
     flags = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC"] + arch + (["-Xptxas", "-v"] if verbose else [])

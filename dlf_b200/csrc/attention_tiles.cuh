@@ -20,6 +20,7 @@
 
 #include "attention_decode.cuh"
 #include "attention_plan.h"
+#include "dependents.cuh"
 #include "ptx.cuh"
 
 namespace dlfb200 {
@@ -174,9 +175,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
     }
     if (warp == 8) {
         __syncwarp();
-        ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512u);
-        ptx::tmem_relinquish();
-        ptx::launch_dependents();  // (in this warp, with the tensor memory in hand: see ptx.cuh)
+        ptx::tmem_alloc_then_dependents(ptx::smem_u32(&tmem_slot), 512u);
     }
     if (warp == 9 && lane == 0) {
         ptx::tma_prefetch_desc(&tmQ);

@@ -14,6 +14,7 @@
 #pragma once
 #include "contraction.cuh"
 #include "contraction_split.cuh"
+#include "dependents.cuh"
 
 namespace dlfb200 {
 
@@ -115,9 +116,7 @@ __global__ void __launch_bounds__(kInt8Threads)
     }
     if (warp == 5) {
         __syncwarp();
-        ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), tmem_cols);
-        ptx::tmem_relinquish();
-        ptx::launch_dependents();  // (in this warp, with the tensor memory in hand: see ptx.cuh)
+        ptx::tmem_alloc_then_dependents(ptx::smem_u32(&tmem_slot), tmem_cols);
     }
     if (warp == 4 && lane == 0) {
         ptx::tma_prefetch_desc(&tmL);
@@ -340,9 +339,7 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
     }
     if (warp == 4) {
         __syncwarp();
-        ptx::tmem_alloc_pair(ptx::smem_u32(&tmem_slot), 512u);
-        ptx::tmem_relinquish_pair();
-        ptx::launch_dependents();  // (in this warp, with the tensor memory in hand: see ptx.cuh)
+        ptx::tmem_alloc_pair_then_dependents(ptx::smem_u32(&tmem_slot), 512u);
     }
     if (warp == 5 && lane == 0) {
         ptx::tma_prefetch_desc(&tmA);
