@@ -103,17 +103,15 @@ def _declare(L):
     L.dlf_b200_gemm_int8_workspace_bytes.argtypes = [c_size] * 3 + [c_void, c_size, c_void, c_size]
     L.dlf_b200_attention_workspace_bytes.restype = c_size
     L.dlf_b200_attention_workspace_bytes.argtypes = [c_size] * 6
+    # (the arguments of attention come packed as the structures of the header)
     L.dlf_b200_attention.restype = c_int
-    L.dlf_b200_attention.argtypes = [c_int] + [c_size] * 6 + [ctypes.c_float, c_void, c_void, c_void, c_void, c_void, c_void, c_void,
-                                                              c_void, c_size, c_void, c_void, c_void, c_size, c_void]
+    L.dlf_b200_attention.argtypes = [ctypes.c_char_p, c_void, c_size, c_void]
     L.dlf_b200_paged_attention_workspace_bytes.restype = c_size
     L.dlf_b200_paged_attention_workspace_bytes.argtypes = [c_size] * 4
     L.dlf_b200_paged_attention.restype = c_int
-    L.dlf_b200_paged_attention.argtypes = [c_int] + [c_size] * 4 + [ctypes.c_float] + [c_void] * 6 + [
-        c_size, c_size, c_void, c_size, c_size, c_void, c_void, c_void, c_void, c_size, c_void]
+    L.dlf_b200_paged_attention.argtypes = [ctypes.c_char_p, c_void, c_size, c_void]
     L.dlf_b200_paged_append.restype = c_int
-    L.dlf_b200_paged_append.argtypes = [c_int] + [c_size] * 3 + [c_void] * 8 + [c_size, c_size, c_void, c_size, c_size, c_size,
-                                                                              c_void, c_void, c_void]
+    L.dlf_b200_paged_append.argtypes = [ctypes.c_char_p, c_void]
     L.dlf_b200_status_string.restype = ctypes.c_char_p
     L.dlf_b200_status_string.argtypes = [c_int]
     L.dlf_b200_device_status.restype = c_int

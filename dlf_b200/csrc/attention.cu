@@ -16,9 +16,8 @@ using namespace dlfb200;
 
 namespace {
 
-constexpr int kDecodeCtasPerSm = 2;
 constexpr int kDecodeLeast = 2;    // units a CTA takes at least
-constexpr long long kB200Sms = 148;  // for sizes that are asked for without a device at hand
+constexpr int kB200Sms = 148;  // for sizes that are asked for without a device at hand
 
 struct AttentionDevice {
     bool ready = false;
@@ -28,8 +27,14 @@ std::mutex g_attention_mu;
 
 template <bool BF16, int DP>
 int attention_limits() {
-    CUDA_TRY(cudaFuncSetAttribute(attention_decode_kernel<BF16, DP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(DP)));
-    CUDA_TRY(cudaFuncSetAttribute(attention_decode_kernel<BF16, DP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(DP)));
+    for (auto k : {attention_decode_kernel<BF16, DP, KEYS_PLAIN, 1, true>, attention_decode_kernel<BF16, DP, KEYS_PLAIN, 1, false>,
+                   attention_decode_kernel<BF16, DP, KEYS_PAGES_16, 1, true>, attention_decode_kernel<BF16, DP, KEYS_ANY, 1, true>,
+                   attention_decode_kernel<BF16, DP, KEYS_ANY, 1, false>})
+        CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(DP, 1)));
+    for (auto k : {attention_decode_kernel<BF16, DP, KEYS_PLAIN, 2, true>, attention_decode_kernel<BF16, DP, KEYS_PLAIN, 2, false>,
+                   attention_decode_kernel<BF16, DP, KEYS_PAGES_16, 2, true>, attention_decode_kernel<BF16, DP, KEYS_ANY, 2, true>,
+                   attention_decode_kernel<BF16, DP, KEYS_ANY, 2, false>})
+        CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(DP, 2)));
     CUDA_TRY(cudaFuncSetAttribute(attention_tiles_kernel<BF16, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, tiles_smem(DP)));
     return kSuccess;
 }
@@ -52,24 +57,36 @@ bool strides_ok(std::initializer_list<size_t> s) {
     return true;
 }
 
-size_t decode_workspace(int ctas, size_t size) { return static_cast<size_t>(2 * ctas) * decode_slot(static_cast<int>(size)) * 4; }
+size_t decode_workspace(size_t size) { return static_cast<size_t>(2 * kB200Sms * decode_ctas_per_sm(static_cast<int>(size), 1)) * decode_slot(static_cast<int>(size)) * 4; }
 
-template <bool BF16, int DP, bool PAGED>
+template <bool BF16, int DP, int KEYS, int NB, bool FULL>
 int decode_launch(const DecodeParams& p, cudaStream_t stream) {
-    CUDA_TRY(launch_dependent(attention_decode_kernel<BF16, DP, PAGED>, static_cast<unsigned>(p.ctas), kDecodeThreads, decode_smem(DP), stream, p));
+    CUDA_TRY(launch_dependent(attention_decode_kernel<BF16, DP, KEYS, NB, FULL>, static_cast<unsigned>(p.ctas), kDecodeThreads, decode_smem(DP, NB), stream, p));
     count_launch();
     CUDA_TRY(launch_dependent(attention_join_kernel<BF16>, static_cast<unsigned>(p.batch * p.kv_heads * p.row_blocks), 128u, 0, stream, p));
     count_launch();
     CUDA_TRY(cudaGetLastError());
     return kSuccess;
 }
-int decode_any(const DecodeParams& p, bool bf16, bool paged, cudaStream_t stream) {
-    if (p.size <= 64) {
-        if (bf16) return paged ? decode_launch<true, 64, true>(p, stream) : decode_launch<true, 64, false>(p, stream);
-        return paged ? decode_launch<false, 64, true>(p, stream) : decode_launch<false, 64, false>(p, stream);
-    }
-    if (bf16) return paged ? decode_launch<true, 128, true>(p, stream) : decode_launch<true, 128, false>(p, stream);
-    return paged ? decode_launch<false, 128, true>(p, stream) : decode_launch<false, 128, false>(p, stream);
+template <bool BF16, int DP, int NB>
+int decode_keys(const DecodeParams& p, cudaStream_t stream) {
+    const bool full = p.size == DP;
+    if (p.table != nullptr && full && p.page_size % 16 == 0) return decode_launch<BF16, DP, KEYS_PAGES_16, NB, true>(p, stream);
+    if (p.table != nullptr || p.mask != nullptr)
+        return full ? decode_launch<BF16, DP, KEYS_ANY, NB, true>(p, stream) : decode_launch<BF16, DP, KEYS_ANY, NB, false>(p, stream);
+    return full ? decode_launch<BF16, DP, KEYS_PLAIN, NB, true>(p, stream) : decode_launch<BF16, DP, KEYS_PLAIN, NB, false>(p, stream);
+}
+template <bool BF16, int DP>
+int decode_rows(DecodeParams& p, cudaStream_t stream) {
+    const int rows = p.tokens * p.group;
+    p.block_rows = rows <= 8 ? 8 : 16;
+    p.ctas *= decode_ctas_per_sm(DP, rows <= 8 ? 1 : 2);
+    p.row_blocks = (rows + p.block_rows - 1) / p.block_rows;
+    return rows <= 8 ? decode_keys<BF16, DP, 1>(p, stream) : decode_keys<BF16, DP, 2>(p, stream);
+}
+int decode_any(DecodeParams& p, bool bf16, cudaStream_t stream) {
+    if (p.size <= 64) return bf16 ? decode_rows<true, 64>(p, stream) : decode_rows<false, 64>(p, stream);
+    return bf16 ? decode_rows<true, 128>(p, stream) : decode_rows<false, 128>(p, stream);
 }
 
 // tensor map of a (batch, tokens, heads, size) tensor: boxes of `rows` tokens x 64 values of one head, 128-byte swizzle
@@ -112,20 +129,20 @@ size_t dlf_b200_attention_workspace_bytes(size_t batch, size_t queries, size_t k
     (void)batch;
     (void)keys;
     if (kv_heads == 0 || heads % kv_heads != 0) return 0;
-    return few_rows(queries, heads / kv_heads) ? decode_workspace(kDecodeCtasPerSm * kB200Sms, size) : 0;
+    return few_rows(queries, heads / kv_heads) ? decode_workspace(size) : 0;
 }
 
-int dlf_b200_attention(int dtype, size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size, float scale,
-                       const void* q, const size_t* q_strides, const void* k, const size_t* k_strides, const void* v,
-                       const size_t* v_strides, const int* key_lengths, const unsigned char* key_mask, size_t key_mask_ld, void* y,
-                       const size_t* y_strides, void* workspace, size_t workspace_bytes, void* stream) {
+int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+    if (args == nullptr) return kInvalidValue;
+    const auto& [dtype, scale, batch, queries, keys, heads, kv_heads, size, q_strides, k_strides, v_strides, y_strides, key_mask_ld, q, k, v, y,
+                 key_lengths, key_mask] = *args;
     int rc = head_args(dtype, heads, kv_heads, size);
     if (rc != kSuccess) return rc;
     if (batch == 0 || queries == 0 || keys == 0 || batch > 65535 || queries > INT_MAX / 2 || keys > INT_MAX / 2) return kInvalidDimension;
     if (!(scale > 0.0f) || std::isinf(scale)) return kInvalidValue;
-    if (q == nullptr || q_strides == nullptr) return kInvalidMatrixA;
-    if (k == nullptr || v == nullptr || k_strides == nullptr || v_strides == nullptr) return kInvalidMatrixB;
-    if (y == nullptr || y_strides == nullptr) return kInvalidMatrixC;
+    if (q == nullptr) return kInvalidMatrixA;
+    if (k == nullptr || v == nullptr) return kInvalidMatrixB;
+    if (y == nullptr) return kInvalidMatrixC;
     if (key_mask != nullptr && key_mask_ld < keys && batch > 1) return kInvalidLeadDimB;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(y) ||
         !strides_ok({q_strides[0], q_strides[1], q_strides[2], k_strides[0], k_strides[1], k_strides[2], v_strides[0], v_strides[1], v_strides[2],
@@ -171,13 +188,12 @@ int dlf_b200_attention(int dtype, size_t batch, size_t queries, size_t keys, siz
         p.group = static_cast<int>(group);
         p.size = static_cast<int>(size);
         p.keys = static_cast<int>(keys);
-        p.row_blocks = static_cast<int>((queries * group + 15) / 16);
-        p.ctas = std::min(kDecodeCtasPerSm * dev.num_sms, static_cast<int>(kDecodeCtasPerSm * kB200Sms));
+        p.ctas = std::min(dev.num_sms, kB200Sms);
         p.least = kDecodeLeast;
         p.c = c;
         p.parts = static_cast<float*>(workspace);
         p.status = dev.status;
-        return decode_any(p, bf16, false, s);
+        return decode_any(p, bf16, s);
     }
     TilesParams p{};
     p.batch = static_cast<int>(batch);
@@ -215,24 +231,23 @@ size_t dlf_b200_paged_attention_workspace_bytes(size_t batch, size_t heads, size
     (void)batch;
     (void)heads;
     (void)kv_heads;
-    return decode_workspace(kDecodeCtasPerSm * kB200Sms, size);
+    return decode_workspace(size);
 }
 
-int dlf_b200_paged_attention(int dtype, size_t batch, size_t heads, size_t kv_heads, size_t size, float scale, const void* q,
-                             const size_t* q_strides, const void* k_pages, const size_t* k_strides, const void* v_pages,
-                             const size_t* v_strides, size_t num_pages, size_t page_size, const int* page_table, size_t table_width,
-                             size_t table_ld, const int* lengths, void* y, const size_t* y_strides, void* workspace, size_t workspace_bytes,
-                             void* stream) {
+int dlf_b200_paged_attention(const dlf_b200_paged_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+    if (args == nullptr) return kInvalidValue;
+    const auto& [dtype, scale, batch, heads, kv_heads, size, num_pages, page_size, table_width, table_ld, q_strides, k_strides, v_strides, y_strides,
+                 q, k_pages, v_pages, y, page_table, lengths] = *args;
     int rc = head_args(dtype, heads, kv_heads, size);
     if (rc != kSuccess) return rc;
     if (batch == 0 || num_pages == 0 || page_size == 0 || table_width == 0 || batch > 65535 || num_pages > INT_MAX || page_size > INT_MAX ||
         static_cast<double>(table_width) * static_cast<double>(page_size) > INT_MAX / 2)
         return kInvalidDimension;
     if (!(scale > 0.0f) || std::isinf(scale)) return kInvalidValue;
-    if (q == nullptr || q_strides == nullptr) return kInvalidMatrixA;
-    if (k_pages == nullptr || v_pages == nullptr || k_strides == nullptr || v_strides == nullptr || page_table == nullptr || lengths == nullptr)
+    if (q == nullptr) return kInvalidMatrixA;
+    if (k_pages == nullptr || v_pages == nullptr || page_table == nullptr || lengths == nullptr)
         return kInvalidMatrixB;
-    if (y == nullptr || y_strides == nullptr) return kInvalidMatrixC;
+    if (y == nullptr) return kInvalidMatrixC;
     if (table_ld < table_width && batch > 1) return kInvalidLeadDimB;
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(y) ||
         !strides_ok({q_strides[0], q_strides[1], k_strides[0], k_strides[1], k_strides[2], v_strides[0], v_strides[1], v_strides[2], y_strides[0],
@@ -270,28 +285,27 @@ int dlf_b200_paged_attention(int dtype, size_t batch, size_t heads, size_t kv_he
     p.group = static_cast<int>(heads / kv_heads);
     p.size = static_cast<int>(size);
     p.keys = static_cast<int>(table_width * page_size);
-    p.row_blocks = (p.group + 15) / 16;
-    p.ctas = std::min(kDecodeCtasPerSm * dev.num_sms, static_cast<int>(kDecodeCtasPerSm * kB200Sms));
+    p.ctas = std::min(dev.num_sms, kB200Sms);
     p.least = kDecodeLeast;
     p.c = scale * 1.44269504088896340736f;
     p.parts = static_cast<float*>(workspace);
     p.status = dev.status;
-    return decode_any(p, dtype == DLF_B200_BFLOAT16, true, s);
+    return decode_any(p, dtype == DLF_B200_BFLOAT16, s);
 }
 
-int dlf_b200_paged_append(int dtype, size_t tokens, size_t kv_heads, size_t size, const void* k, const size_t* k_strides, const void* v,
-                          const size_t* v_strides, void* k_pages, const size_t* kp_strides, void* v_pages, const size_t* vp_strides,
-                          size_t num_pages, size_t page_size, const int* page_table, size_t batch, size_t table_width, size_t table_ld,
-                          const int* positions, const int* sequences, void* stream) {
+int dlf_b200_paged_append(const dlf_b200_paged_append_args* args, void* stream) {
+    if (args == nullptr) return kInvalidValue;
+    const auto& [dtype, tokens, kv_heads, size, batch, num_pages, page_size, table_width, table_ld, k_strides, v_strides, kp_strides, vp_strides, k, v,
+                 k_pages, v_pages, page_table, positions, sequences] = *args;
     int rc = head_args(dtype, kv_heads, kv_heads, size);
     if (rc != kSuccess) return rc;
     if (tokens == 0 || batch == 0 || num_pages == 0 || page_size == 0 || table_width == 0 || tokens > INT_MAX || batch > INT_MAX || num_pages > INT_MAX ||
         page_size > INT_MAX || table_width > INT_MAX || kv_heads * size > INT_MAX)
         return kInvalidDimension;
     if (sequences == nullptr && tokens > batch) return kInvalidDimension;
-    if (k == nullptr || v == nullptr || k_strides == nullptr || v_strides == nullptr) return kInvalidMatrixA;
+    if (k == nullptr || v == nullptr) return kInvalidMatrixA;
     if (page_table == nullptr || positions == nullptr) return kInvalidMatrixB;
-    if (k_pages == nullptr || v_pages == nullptr || kp_strides == nullptr || vp_strides == nullptr) return kInvalidMatrixC;
+    if (k_pages == nullptr || v_pages == nullptr) return kInvalidMatrixC;
     if (table_ld < table_width && batch > 1) return kInvalidLeadDimB;
     if (!aligned16(k) || !aligned16(v) || !aligned16(k_pages) || !aligned16(v_pages) ||
         !strides_ok({k_strides[0], k_strides[1], v_strides[0], v_strides[1], kp_strides[0], kp_strides[1], kp_strides[2], vp_strides[0], vp_strides[1],

@@ -4,18 +4,19 @@
 //     y_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp2(c q_r.k_j - m_r),  c = scale * log2(e),  m_r the largest so far
 //
 // HBM-bound: the keys and values of a kv head are read once for up to 16 query rows (the query heads that share it), so
-// what counts is how many bytes are in flight. A block has four warps; of a unit of 64 keys each takes 16 and runs the
-// recurrence by itself (running maximum and sum, 32-bit accumulators), with its own ring of cp.async copies; the warps meet
-// at the end of a segment (attention_plan.h). Products are mma.m16n8k16: 16 query rows, of which G are used.
+// what counts is how many bytes are in flight and how few instructions a key costs. A block has four warps; of a unit of 64
+// keys each takes 16 and runs the recurrence by itself (running maximum and sum, 32-bit accumulators), with its own ring of
+// cp.async copies; the warps meet at the end of a segment (attention_plan.h).
 //
-// Every lane copies exactly the 16-byte pieces that its own fragments are made of, so a copy is followed by no barrier
-// and read without bank conflicts (piece i of lane l lies at (32 i + l) * 16). With g = lane / 4, t = lane % 4:
-//   K: lane (g, t) takes pieces t + 4 j of keys g and 8 + g. In q.k the head's d's may be taken in any order, so the four words
-//      of a piece are the k-halves of two k-steps, and q's fragments are loaded in the same order.
-//   V: lane (g, t) takes pieces g + 8 j of keys 2t, 2t+1, 2t+8, 2t+9 - the keys of its fragments - and pairs two keys'
-//      words for each of the piece's eight d's; accumulator column n of n-tile (j, e) is then d = 8 (n + 8 j) + e.
-// p is rounded to 16 bits for the second product in two parts (its rounding and the rest), which costs no time here and keeps
-// the result as exact as 32-bit arithmetic.
+// Products are mma.m16n8k16 with the keys (or the head's d's) as the 16 rows and the queries as the 8 columns, so up to
+// eight query rows cost one set of instructions, up to 16 two (NB):
+//   S^T = K Q^T: with g = lane / 4, t = lane % 4, lane (g, t) copies the 16-byte pieces t + 4 j of keys g and 8 + g and reads back
+//      the same pieces: their four words are its fragments of two k-steps, if q's are taken in the same order of d's (a sum
+//      over d has no order). No exchange, no bank conflicts.
+//   O^T += V^T P^T: V's fragments by ldmatrix.trans (lines swizzled by the key), P^T by movmatrix from S^T's accumulators.
+// The maximum of a row is moved (and O scaled) only when a score exceeds it by more than 2^8; until then a step needs no exchange
+// between lanes. p is rounded to 16 bits for the second product in two parts (its rounding and the rest), so that the result is as
+// exact as 32-bit arithmetic makes it.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -41,18 +42,26 @@ struct DecodeParams {
     long long table_sb;
     int page_size, num_pages;
     int batch, tokens, kv_heads, group, size, keys;
-    int row_blocks;                                // blocks of 16 rows (row = token * group + head of the group)
+    int row_blocks, block_rows;                    // blocks of 8 or 16 rows (row = token * group + head of the group)
     int ctas, least;
     float c;                                       // scale * log2(e)
     float* parts;                                  // slots of 16 x (size + 2) floats: sums, then maximum and sum of p per row
     int* status;
 };
 
+// where a sequence's keys lie: one after the other; in pages of a multiple of 16 tokens (a step's 16 keys lie in one page); in
+// pages of any size, or under a mask (every key by itself)
+enum : int { KEYS_PLAIN = 0, KEYS_PAGES_16 = 1, KEYS_ANY = 2 };
+
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeWarps = kDecodeThreads / 32;
-DLF_HD constexpr int decode_stages(int dp) { return dp <= 64 ? 6 : 3; }
+// Stages of a warp's ring and blocks of an SM: nb = 1 or 2 sets of eight query rows. More blocks with shorter rings carry short
+// segments better (32 sequences of up to 1500 keys, 16 heads of 64: 4 blocks of 3 stages 27.8 us, 3 of 4 29.2, 2 of 6 33.3), and cost long
+// ones nothing (64 of up to 8192 keys, 8 heads of 128: 3 blocks of 2 stages 182.5 us, 2 of 3 184.4).
+DLF_HD constexpr int decode_ctas_per_sm(int dp, int nb) { return dp <= 64 ? (nb == 1 ? 4 : 3) : (nb == 1 ? 3 : 2); }
+DLF_HD constexpr int decode_stages(int dp, int nb) { return dp <= 64 ? (nb == 1 ? 3 : 4) : (nb == 1 ? 2 : 3); }
 DLF_HD constexpr int decode_stage_bytes(int dp) { return 16 * dp * 2 * 2; }  // a warp's 16 keys and values
-DLF_HD constexpr int decode_smem(int dp) { return kDecodeWarps * decode_stages(dp) * decode_stage_bytes(dp); }
+DLF_HD constexpr int decode_smem(int dp, int nb) { return kDecodeWarps * decode_stages(dp, nb) * decode_stage_bytes(dp); }
 DLF_HD constexpr int decode_slot(int size) { return 16 * (size + 2); }
 
 namespace ptx {
@@ -73,6 +82,18 @@ __device__ __forceinline__ uint4 lds_128(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
     return v;
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t (&v)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed_8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
 }
 template <bool BF16>
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -161,18 +182,23 @@ __device__ __forceinline__ int decode_find(const DecodeParams& p, long long u, i
     return p.batch;
 }
 
-template <bool BF16, int DP, bool PAGED>
-__global__ void __launch_bounds__(kDecodeThreads) attention_decode_kernel(const __grid_constant__ DecodeParams p) {
-    constexpr int STAGES = decode_stages(DP);
-    constexpr int PK = DP / 32;  // pieces of a key per lane (key g: t + 4 j, j < PK)
-    constexpr int PV = DP / 64;  // pieces of a value per lane (g + 8 j, j < PV)
-    constexpr int STAGE = decode_stage_bytes(DP);
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+template <bool BF16, int DP, int KEYS, int NB, bool FULL>  // FULL: the head has all DP values
+__global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) attention_decode_kernel(const __grid_constant__ DecodeParams p) {
+    constexpr int STAGES = decode_stages(DP, NB);
+    constexpr int PK = DP / 32;  // pieces of a key per lane: t + 4 j, j < PK
+    constexpr int PV = DP / 64;  // pieces of a value per lane: lane % 8 + 8 j
+    constexpr int STAGE = decode_stage_bytes(DP), VOFF = STAGE / 2, LINE = DP * 2;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t ring = ptx::smem_u32(smem_raw) + warp * STAGES * STAGE + lane * 16;
+    const uint32_t ring = ptx::smem_u32(smem_raw) + warp * STAGES * STAGE;
+    // V: copied as piece lane % 8 + 8 j of keys lane / 8 + 4 i, to line `key`, piece ^ (key % 8)
+    const int vkey = lane >> 3, vch = lane & 7;
+    // read by ldmatrix: lane's line is key (lane & 7) + 8 for lanes 16.., piece + 1 for lanes 8-15 and 24-31
+    const int mkey = (lane & 7) + ((lane >> 4) << 3), mch = (lane >> 3) & 1;
+    const uint32_t vread = VOFF + mkey * LINE;
 
-    ptx::launch_dependents();
     ptx::wait_for_dependencies();
+    ptx::launch_dependents();  // (behind the wait: what runs before this kernel is done when the joining one starts)
 
     const int heads = p.kv_heads * p.row_blocks;
     long long before, all;
@@ -188,89 +214,133 @@ __global__ void __launch_bounds__(kDecodeThreads) attention_decode_kernel(const 
     int hb = static_cast<int>((u - before) / units);       // head and row block
     int unit0 = static_cast<int>(u - before - static_cast<long long>(hb) * units);
     const int chunks = p.size / 8;
+    const float c = p.c, limit = 8.0f / c;
     bool bad_page = false;
 
     while (u < end) {
         const int n_units = static_cast<int>(min(static_cast<long long>(units - unit0), end - u));
         const bool whole = n_units == units;
         const int slot = plan_slot(u, per);
-        const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * 16;
-        const int rows = min(16, p.tokens * p.group - row0);
-        // ---------------------------------------------------------------- q
-        uint32_t qf[2 * PK][4];
-        auto q_piece = [&](int r, int j) -> uint4 {
-            const int row = row0 + r, ch = t + 4 * j;
-            if (r >= rows || ch >= chunks) return make_uint4(0u, 0u, 0u, 0u);
-            const int tok = row / p.group, h = hk * p.group + row - tok * p.group;
-            return *reinterpret_cast<const uint4*>(p.q + (b * p.q_sb + tok * p.q_st + h * p.q_sh + ch * 8) * 2);
-        };
-#pragma unroll
-        for (int j = 0; j < PK; ++j) {
-            const uint4 lo = q_piece(g, j), hi = q_piece(g + 8, j);
-            qf[2 * j][0] = lo.x, qf[2 * j][1] = hi.x, qf[2 * j][2] = lo.y, qf[2 * j][3] = hi.y;
-            qf[2 * j + 1][0] = lo.z, qf[2 * j + 1][1] = hi.z, qf[2 * j + 1][2] = lo.w, qf[2 * j + 1][3] = hi.w;
-        }
+        const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * p.block_rows;
+        const int rows = min(8 * NB, p.tokens * p.group - row0);
         // ---------------------------------------------------------------- copies
-        // step i of this warp: keys first_key + 64 i .. + 15 of the segment's units
+        // step i of this warp: keys first_key + 64 i .. + 15
         const int first_key = unit0 * kPlanUnit + warp * 16;
-        const char* kbase = p.k + (PAGED ? 0 : b * p.k_sb * 2) + hk * p.k_sh * 2;
-        const char* vbase = p.v + (PAGED ? 0 : b * p.v_sb * 2) + hk * p.v_sh * 2;
-        const unsigned char* mask = p.mask != nullptr ? p.mask + b * p.mask_sb : nullptr;
-        // lane l < 16 finds where key l of a step lies: its place in the cache (or its position), -1 = not kept
-        auto find_row = [&](int i) -> long long {
-            const int pos = first_key + i * kPlanUnit + (lane & 15);
-            if (i >= n_units || pos >= len) return -1;
-            if constexpr (PAGED) {
-                const int pg = pos / p.page_size, place = pos - pg * p.page_size;
-                const long long row = plan_place(p.table[b * p.table_sb + pg], place, p.num_pages);
-                if (row < 0) bad_page = true;
-                return row;
-            } else {
-                return mask != nullptr && mask[pos] == 0 ? -1 : pos;
+        const long long kst = p.k_st * 2, vst = p.v_st * 2;  // bytes between tokens
+        const char* kbase = p.k + (p.table != nullptr ? 0 : b * p.k_sb * 2) + hk * p.k_sh * 2 + t * 16;
+        const char* vbase = p.v + (p.table != nullptr ? 0 : b * p.v_sb * 2) + hk * p.v_sh * 2 + vch * 16;
+        // what a step needs to know before it can be fetched: KEYS_PAGES_16 its page, KEYS_ANY lane l < 16 the place of key l (-1: not
+        // kept). Asked for a step ahead of the fetch.
+        auto ask = [&](int i) -> long long {
+            const int pos = first_key + i * kPlanUnit + (KEYS == KEYS_ANY ? (lane & 15) : 0);
+            if (KEYS == KEYS_PLAIN || i >= n_units || pos >= len) return -1;
+            if (KEYS == KEYS_PAGES_16 || p.table != nullptr) {
+                const int pg = pos / p.page_size;
+                const long long at = plan_place(p.table[b * p.table_sb + pg], pos - pg * p.page_size, p.num_pages);
+                if (at < 0) bad_page = true;
+                return at;
             }
+            return p.mask[b * p.mask_sb + pos] == 0 ? -1 : pos;
         };
-        auto offset_of = [&](long long row, long long sb, long long st) -> long long {  // bytes
-            if constexpr (PAGED) {
-                return ((row >> 32) * sb + static_cast<int>(row) * st) * 2;
-            } else {
-                return row * st * 2;
-            }
-        };
-        auto fetch = [&](int stage, long long row) {
-            const uint32_t at = ring + stage * STAGE;
-            const long long ko = row >= 0 ? offset_of(row, p.k_sb, p.k_st) : -1, vo = row >= 0 ? offset_of(row, p.v_sb, p.v_st) : -1;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const long long o = __shfl_sync(0xffffffffu, ko, n * 8 + g);
-#pragma unroll
-                for (int j = 0; j < PK; ++j) {
-                    const bool ok = o >= 0 && t + 4 * j < chunks;
-                    ptx::cp_async_16(at + (n * PK + j) * 512, kbase + (ok ? o + (t + 4 * j) * 16 : 0), ok);
+        // step i to a stage; returns which of its 16 keys count
+        auto fetch = [&](int stage, int i, long long at) -> unsigned {
+            const uint32_t kdst = ring + stage * STAGE + lane * 16;
+            const uint32_t vdst = ring + stage * STAGE + VOFF + vkey * LINE;
+            const int left = len - (first_key + i * kPlanUnit);
+            if constexpr (KEYS != KEYS_ANY) {
+                const char* kp = kbase + g * kst;
+                const char* vp = vbase + vkey * vst;
+                if constexpr (KEYS == KEYS_PAGES_16) {
+                    kp += ((at >> 32) * p.k_sb + static_cast<int>(at) * p.k_st) * 2;
+                    vp += ((at >> 32) * p.v_sb + static_cast<int>(at) * p.v_st) * 2;
+                } else {
+                    kp += (first_key + static_cast<long long>(i) * kPlanUnit) * kst;
+                    vp += (first_key + static_cast<long long>(i) * kPlanUnit) * vst;
                 }
-            }
+                if (FULL && left >= 16 && (KEYS == KEYS_PLAIN || at >= 0)) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const long long o = __shfl_sync(0xffffffffu, vo, (n >> 1) * 8 + 2 * t + (n & 1));
+                    for (int n = 0; n < 2; ++n)
 #pragma unroll
-                for (int j = 0; j < PV; ++j) {
-                    const bool ok = o >= 0 && g + 8 * j < chunks;
-                    ptx::cp_async_16(at + (2 * PK + n * PV + j) * 512, vbase + (ok ? o + (g + 8 * j) * 16 : 0), ok);
+                        for (int j = 0; j < PK; ++j) ptx::cp_async_16(kdst + (n * PK + j) * 512, kp + n * 8 * kst + j * 64);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n)
+#pragma unroll
+                        for (int j = 0; j < PV; ++j) ptx::cp_async_16(vdst + n * 4 * LINE + (((vch + 8 * j) ^ ((vkey + 4 * n) & 7)) << 4), vp + n * 4 * vst + j * 128);
+                    return 0xffffu;
                 }
+                const int keys = (KEYS == KEYS_PLAIN || at >= 0) ? max(min(left, 16), 0) : 0;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int j = 0; j < PK; ++j) {
+                        const bool ok = n * 8 + g < keys && (FULL || t + 4 * j < chunks);
+                        ptx::cp_async_16(kdst + (n * PK + j) * 512, ok ? kp + n * 8 * kst + j * 64 : p.k, ok);
+                    }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int j = 0; j < PV; ++j) {
+                        const bool ok = n * 4 + vkey < keys && (FULL || vch + 8 * j < chunks);
+                        ptx::cp_async_16(vdst + n * 4 * LINE + (((vch + 8 * j) ^ ((vkey + 4 * n) & 7)) << 4), ok ? vp + n * 4 * vst + j * 128 : p.v, ok);
+                    }
+                return (1u << keys) - 1u;
+            } else {
+                const bool paged = p.table != nullptr;
+                const long long ko = at < 0 ? -1 : paged ? ((at >> 32) * p.k_sb + static_cast<int>(at) * p.k_st) * 2 : at * kst;
+                const long long vo = at < 0 ? -1 : paged ? ((at >> 32) * p.v_sb + static_cast<int>(at) * p.v_st) * 2 : at * vst;
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const long long o = __shfl_sync(0xffffffffu, ko, n * 8 + g);
+#pragma unroll
+                    for (int j = 0; j < PK; ++j) {
+                        const bool ok = o >= 0 && (FULL || t + 4 * j < chunks);
+                        ptx::cp_async_16(kdst + (n * PK + j) * 512, ok ? kbase + o + j * 64 : p.k, ok);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const long long o = __shfl_sync(0xffffffffu, vo, n * 4 + vkey);
+#pragma unroll
+                    for (int j = 0; j < PV; ++j) {
+                        const bool ok = o >= 0 && (FULL || vch + 8 * j < chunks);
+                        ptx::cp_async_16(vdst + n * 4 * LINE + (((vch + 8 * j) ^ ((vkey + 4 * n) & 7)) << 4), ok ? vbase + o + j * 128 : p.v, ok);
+                    }
+                }
+                return __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
             }
         };
-        float o[8 * PV][4];
-#pragma unroll
-        for (int i = 0; i < 8 * PV; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
         unsigned kept[STAGES];  // which of a stage's 16 keys count
-        long long next = find_row(0);
+        long long next = ask(0);
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
-            const long long row = next;
-            next = find_row(s + 1);
-            kept[s] = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-            if (s < n_units) fetch(s, row);
+            const long long at = next;
+            next = ask(s + 1);
+            kept[s] = 0u;
+            if (s < n_units) kept[s] = fetch(s, s, at);
             ptx::cp_async_commit();
+        }
+        // ---------------------------------------------------------------- q: fragments of columns (queries) 8 nb + g
+        uint32_t qf[NB][2 * PK][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int j = 0; j < PK; ++j) {
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                const int r = nb * 8 + g, row = row0 + r;
+                if (r < rows && (FULL || t + 4 * j < chunks)) {
+                    const int tok = row / p.group, h = hk * p.group + row - tok * p.group;
+                    w = *reinterpret_cast<const uint4*>(p.q + (b * p.q_sb + tok * p.q_st + h * p.q_sh + (t + 4 * j) * 8) * 2);
+                }
+                qf[nb][2 * j][0] = w.x, qf[nb][2 * j][1] = w.y, qf[nb][2 * j + 1][0] = w.z, qf[nb][2 * j + 1][1] = w.w;
+            }
+        float o[NB][DP / 16][4];
+        float m[NB][2], l[NB][2];  // queries 8 nb + 2 t and + 1
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int x = 0; x < DP / 16; ++x) o[nb][x][0] = o[nb][x][1] = o[nb][x][2] = o[nb][x][3] = 0.0f;
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.0f;
         }
         // ---------------------------------------------------------------- keys
         for (int i0 = 0; i0 < n_units; i0 += STAGES) {
@@ -278,116 +348,119 @@ __global__ void __launch_bounds__(kDecodeThreads) attention_decode_kernel(const 
             for (int s = 0; s < STAGES; ++s) {
                 const int i = i0 + s;
                 if (i < n_units) {
+                    ptx::cp_async_wait<STAGES - 2>();
+                    __syncwarp();  // the other lanes' copies too; and what is filled next has been read by every lane
                     {
                         constexpr int A = STAGES - 1;
-                        const long long row = next;
-                        next = find_row(i + A + 1);
-                        kept[(s + A) % STAGES] = __ballot_sync(0xffffffffu, row >= 0) & 0xffffu;
-                        if (i + A < n_units) fetch((s + A) % STAGES, row);
+                        const long long at = next;
+                        next = ask(i + A + 1);
+                        if (i + A < n_units) kept[(s + A) % STAGES] = fetch((s + A) % STAGES, i + A, at);
                         ptx::cp_async_commit();
                     }
-                    ptx::cp_async_wait<STAGES - 1>();
-                    const uint32_t at = ring + s * STAGE;
-                    float sc[2][4];
+                    const uint32_t st = ring + s * STAGE;
+                    float sc[NB][4];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
+                    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.0f;
 #pragma unroll
-                        for (int j = 0; j < PK; ++j) {
-                            const uint4 kk = ptx::lds_128(at + (n * PK + j) * 512);
-                            ptx::mma_16816<BF16>(sc[n], qf[2 * j][0], qf[2 * j][1], qf[2 * j][2], qf[2 * j][3], kk.x, kk.y);
-                            ptx::mma_16816<BF16>(sc[n], qf[2 * j + 1][0], qf[2 * j + 1][1], qf[2 * j + 1][2], qf[2 * j + 1][3], kk.z, kk.w);
+                    for (int j = 0; j < PK; ++j) {
+                        const uint4 lo = ptx::lds_128(st + lane * 16 + j * 512), hi = ptx::lds_128(st + lane * 16 + (PK + j) * 512);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            ptx::mma_16816<BF16>(sc[nb], lo.x, hi.x, lo.y, hi.y, qf[nb][2 * j][0], qf[nb][2 * j][1]);
+                            ptx::mma_16816<BF16>(sc[nb], lo.z, hi.z, lo.w, hi.w, qf[nb][2 * j + 1][0], qf[nb][2 * j + 1][1]);
                         }
                     }
                     const unsigned kp = kept[s];
-                    float mx[2] = {-INFINITY, -INFINITY};
+                    if (kp != 0xffffu) {
+                        const bool lo = (kp >> g) & 1u, hi = (kp >> (8 + g)) & 1u;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool in = (kp >> (n * 8 + 2 * t + (e & 1))) & 1u;
-                            sc[n][e] = in ? sc[n][e] * p.c : -INFINITY;
-                            mx[e >> 1] = fmaxf(mx[e >> 1], sc[n][e]);
+                        for (int nb = 0; nb < NB; ++nb) {
+                            if (!lo) sc[nb][0] = sc[nb][1] = -INFINITY;
+                            if (!hi) sc[nb][2] = sc[nb][3] = -INFINITY;
                         }
+                    }
                     bool grew = false;
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                        grew |= mx[r] > m[r];
-                    }
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) grew |= fmaxf(sc[nb][r], sc[nb][2 + r]) > m[nb][r] + limit;
                     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const float m_new = fmaxf(m[r], mx[r]);
-                            const float f = m_new == -INFINITY ? 1.0f : ptx::exp2_approx(m[r] - m_new);
-                            m[r] = m_new;
-                            l[r] *= f;
+                        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                            for (int x = 0; x < 8 * PV; ++x) {
-                                o[x][2 * r] *= f;
-                                o[x][2 * r + 1] *= f;
+                            for (int r = 0; r < 2; ++r) {
+                                float x = fmaxf(fmaxf(sc[nb][r], sc[nb][2 + r]), m[nb][r]);
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                                const float f = x == m[nb][r] ? 1.0f : ptx::exp2_approx((m[nb][r] - x) * c);
+                                m[nb][r] = x;
+                                l[nb][r] *= f;
+#pragma unroll
+                                for (int y = 0; y < DP / 16; ++y) {
+                                    o[nb][y][r] *= f;
+                                    o[nb][y][2 + r] *= f;
+                                }
                             }
+                    }
+                    uint32_t ph[NB][2], pl[NB][2];  // P^T fragments: keys 0-7 and 8-15
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        float e[4];
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float mc = m[nb][r] == -INFINITY ? 0.0f : m[nb][r] * c;
+                            e[r] = ptx::exp2_approx(fmaf(sc[nb][r], c, -mc));
+                            e[2 + r] = ptx::exp2_approx(fmaf(sc[nb][2 + r], c, -mc));
+                            l[nb][r] += e[r] + e[2 + r];
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t w = pack_16<BF16>(e[2 * h], e[2 * h + 1]);
+                            const float2 f = unpack_16<BF16>(w);
+                            ph[nb][h] = ptx::transposed_8x8(w);
+                            pl[nb][h] = ptx::transposed_8x8(pack_16<BF16>(e[2 * h] - f.x, e[2 * h + 1] - f.y));
                         }
                     }
-                    const float ms[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-                    uint32_t ph[4], pl[4];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
+                    for (int x = 0; x < DP / 16; ++x) {
+                        uint32_t v[4];
+                        ptx::ldmatrix_x4_trans(st + vread + (((2 * x + mch) ^ (mkey & 7)) << 4), v);
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            const float x = ptx::exp2_approx(sc[n][2 * r] - ms[r]), y = ptx::exp2_approx(sc[n][2 * r + 1] - ms[r]);
-                            l[r] += x + y;
-                            ph[n * 2 + r] = pack_16<BF16>(x, y);
-                            const float2 h = unpack_16<BF16>(ph[n * 2 + r]);
-                            pl[n * 2 + r] = pack_16<BF16>(x - h.x, y - h.y);
-                        }
-#pragma unroll
-                    for (int j = 0; j < PV; ++j) {
-                        const uint4 v0 = ptx::lds_128(at + (2 * PK + 0 * PV + j) * 512), v1 = ptx::lds_128(at + (2 * PK + 1 * PV + j) * 512);
-                        const uint4 v2 = ptx::lds_128(at + (2 * PK + 2 * PV + j) * 512), v3 = ptx::lds_128(at + (2 * PK + 3 * PV + j) * 512);
-                        const uint32_t w0[4] = {v0.x, v0.y, v0.z, v0.w}, w1[4] = {v1.x, v1.y, v1.z, v1.w};
-                        const uint32_t w2[4] = {v2.x, v2.y, v2.z, v2.w}, w3[4] = {v3.x, v3.y, v3.z, v3.w};
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-                            const uint32_t b0 = __byte_perm(w0[e >> 1], w1[e >> 1], sel), b1 = __byte_perm(w2[e >> 1], w3[e >> 1], sel);
-                            ptx::mma_16816<BF16>(o[j * 8 + e], ph[0], ph[1], ph[2], ph[3], b0, b1);
-                            ptx::mma_16816<BF16>(o[j * 8 + e], pl[0], pl[1], pl[2], pl[3], b0, b1);
+                        for (int nb = 0; nb < NB; ++nb) {
+                            ptx::mma_16816<BF16>(o[nb][x], v[0], v[1], v[2], v[3], ph[nb][0], ph[nb][1]);
+                            ptx::mma_16816<BF16>(o[nb][x], v[0], v[1], v[2], v[3], pl[nb][0], pl[nb][1]);
                         }
                     }
                 }
             }
         }
         // ---------------------------------------------------------------- the four warps' results
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        }
         ptx::cp_async_wait<0>();
-        __syncthreads();  // the rings are free: [warp][16 rows][DP + 4] sums, then [warp][16][2] maximum and sum
+        __syncthreads();  // the rings are free: [warp][16 rows][DP + 4] sums, then [warp][16][2] maximum (times c) and sum
         float* sums = reinterpret_cast<float*>(smem_raw);
         float* stat = sums + kDecodeWarps * 16 * (DP + 4);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int row = g + 8 * r;
-            if (row < rows) {
-                float* to = sums + (warp * 16 + row) * (DP + 4);
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int j = 0; j < PV; ++j)
+            for (int r = 0; r < 2; ++r) {
+                float s = l[nb][r];
+                s += __shfl_xor_sync(0xffffffffu, s, 4);
+                s += __shfl_xor_sync(0xffffffffu, s, 8);
+                s += __shfl_xor_sync(0xffffffffu, s, 16);
+                const int row = nb * 8 + 2 * t + r;
+                if (row >= rows) continue;
+                float* to = sums + (warp * 16 + row) * (DP + 4) + g;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-#pragma unroll
-                        for (int e = 0; e < 8; e += 4)
-                            *reinterpret_cast<float4*>(to + (2 * t + n + 8 * j) * 8 + e) =
-                                make_float4(o[j * 8 + e][2 * r + n], o[j * 8 + e + 1][2 * r + n], o[j * 8 + e + 2][2 * r + n], o[j * 8 + e + 3][2 * r + n]);
-                if (t == 0) {
-                    stat[(warp * 16 + row) * 2] = m[r];
-                    stat[(warp * 16 + row) * 2 + 1] = l[r];
+                for (int x = 0; x < DP / 16; ++x) {
+                    to[16 * x] = o[nb][x][r];
+                    to[16 * x + 8] = o[nb][x][2 + r];
+                }
+                if (g == 0) {
+                    stat[(warp * 16 + row) * 2] = m[nb][r] * c;
+                    stat[(warp * 16 + row) * 2 + 1] = s;
                 }
             }
-        }
         __syncthreads();
         float* part = p.parts + static_cast<long long>(slot) * decode_slot(p.size);
         for (int id = threadIdx.x; id < rows * chunks; id += kDecodeThreads) {
@@ -441,16 +514,17 @@ template <bool BF16>
 __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ DecodeParams p) {
     const int heads = p.kv_heads * p.row_blocks;
     const int b = blockIdx.x / heads, hb = blockIdx.x - b * heads;
-    ptx::wait_for_dependencies();
+    // the lengths are those the kernel before this one has read, which it lets this one start behind
     long long before, all;
     decode_units(p, b, before, all);
     const long long per = plan_per(all * heads, p.ctas, p.least);
     const int units = plan_units(decode_length(p, b));
     const long long first = before * heads + static_cast<long long>(hb) * units, last = first + units - 1;
     const int c0 = static_cast<int>(first / per), c1 = static_cast<int>(last / per);
+    const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * p.block_rows;
+    const int rows = min(p.block_rows, p.tokens * p.group - row0), chunks = p.size / 4;
+    ptx::wait_for_dependencies();
     if (c0 == c1) return;
-    const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * 16;
-    const int rows = min(16, p.tokens * p.group - row0), chunks = p.size / 4;
     const long long slot_floats = decode_slot(p.size);
     const float* first_part = p.parts + plan_slot(first, per) * slot_floats;
     for (int id = threadIdx.x; id < rows * chunks; id += blockDim.x) {

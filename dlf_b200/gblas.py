@@ -365,10 +365,7 @@ def quantizeRows(m, n, x_buffer, x_offset, x_ld, q_buffer, q_offset, q_ld, scale
     """Row i of X (m x n) to 8-bit integers in Q and the scale in scales[i] that they are to be multiplied with:
     scales[i] = max |X[i]| / 127 and Q[i] = X[i] / scales[i], rounded to the nearest whole number (ties to even). A row that
     holds an infinity or a NaN gets the scale NaN and zeros."""
-    _quantize_rows(m, n, _buffer_operand(x_buffer, x_offset), x_ld, _buffer_operand(q_buffer, q_offset), q_ld, scales, queue, event)
-
-
-def _quantize_rows(m, n, x, x_ld, q, q_ld, scales, queue=None, event=None):
+    x, q = _buffer_operand(x_buffer, x_offset), _buffer_operand(q_buffer, q_offset)
     prec = precision_of(x)
     if q.dtype != torch.int8 or scales.dtype != torch.float32:
         raise BLASError(StatusCode.kInvalidValue)
@@ -380,11 +377,16 @@ def _quantize_rows(m, n, x, x_ld, q, q_ld, scales, queue=None, event=None):
         raise BLASError(StatusCode.kInsufficientMemoryC)
     if not (x.is_cuda and x.device == q.device == scales.device):
         raise BLASError(StatusCode.kInvalidMatrixA)
-    handle = _operator_stream(queue, x.device)
+    _quantize_rows(int(prec), m, n, x.address, x_ld, q.address, q_ld, scales.data_ptr(), x.device, queue, event)
+
+
+def _quantize_rows(prec, m, n, x, x_ld, q, q_ld, scales, device, queue=None, event=None):
+    """The call itself, with addresses."""
+    handle = _operator_stream(queue, device)
     if event is not None:
         s = queue if queue is not None else torch.cuda.current_stream()
         event.start.record(s)
-    rc = lib().dlf_b200_quantize_rows(int(prec), m, n, x.address, x_ld, q.address, q_ld, scales.data_ptr(), handle)
+    rc = lib().dlf_b200_quantize_rows(prec, m, n, x, x_ld, q, q_ld, scales, handle)
     if event is not None:
         event.end.record(s)
     _check(rc)
@@ -394,11 +396,7 @@ def gemmInt8(m, n, k, a_buffer, a_offset, a_ld, a_scales, b_buffer, b_offset, b_
              activation=None, queue=None, event=None):
     """C[i][j] = act((sum_k A[i][k] * B[j][k]) * b_scales[j] * a_scales[i] + bias[j]): A (m x k) and B (n x k) 8-bit
     integers, row-major, a scale for each of their rows; C (m x n) float16, bfloat16 or float32. The sums are exact."""
-    _gemm_int8(m, n, k, _buffer_operand(a_buffer, a_offset), a_ld, a_scales, _buffer_operand(b_buffer, b_offset), b_ld, b_scales,
-               _buffer_operand(c_buffer, c_offset), c_ld, bias, activation, queue, event)
-
-
-def _gemm_int8(m, n, k, a, a_ld, a_scales, b, b_ld, b_scales, c, c_ld, bias=None, activation=None, queue=None, event=None):
+    a, b, c = _buffer_operand(a_buffer, a_offset), _buffer_operand(b_buffer, b_offset), _buffer_operand(c_buffer, c_offset)
     prec = precision_of(c)
     if (a.dtype != torch.int8 or b.dtype != torch.int8 or a_scales.dtype != torch.float32 or b_scales.dtype != torch.float32 or
             (bias is not None and bias.dtype != c.dtype) or activation not in (None, "relu")):
@@ -417,22 +415,41 @@ def _gemm_int8(m, n, k, a, a_ld, a_scales, b, b_ld, b_scales, c, c_ld, bias=None
     device = c.device
     if not c.is_cuda or any(t.device != device for t in (a, b, a_scales, b_scales)) or (bias is not None and bias.device != device):
         raise BLASError(StatusCode.kInvalidMatrixA)
+    _gemm_int8(int(prec), m, n, k, a.address, a_ld, a_scales.data_ptr(), b.address, b_ld, b_scales.data_ptr(),
+               bias.data_ptr() if bias is not None else None, 1 if activation == "relu" else 0, c.address, c_ld, device, queue, event)
+
+
+def _gemm_int8(prec, m, n, k, a, a_ld, a_scales, b, b_ld, b_scales, bias, activation, c, c_ld, device, queue=None, event=None):
+    """The call itself, with addresses."""
     L = lib()
     handle = _operator_stream(queue, device)
-    need = L.dlf_b200_gemm_int8_workspace_bytes(m, n, k, a.address, a_ld, b.address, b_ld)
-    ws, entry = _operator_scratch(_INT8_WORKSPACES, need, device, queue, handle) if need else (None, None)
+    ws, entry, need = None, None, 0
+    if (a | b) & 15 or (a_ld | b_ld) & 15:  # operands that may have to be copied first (not those of one line)
+        need = L.dlf_b200_gemm_int8_workspace_bytes(m, n, k, a, a_ld, b, b_ld)
+        if need:
+            ws, entry = _operator_scratch(_INT8_WORKSPACES, need, device, queue, handle)
     with entry.lock if entry is not None else _NO_LOCK:
         if entry is not None:
             ws = entry.at_least(need, device, queue)
         if event is not None:
             s = queue if queue is not None else torch.cuda.current_stream()
             event.start.record(s)
-        rc = L.dlf_b200_gemm_int8(int(prec), m, n, k, a.address, a_ld, a_scales.data_ptr(), b.address, b_ld, b_scales.data_ptr(),
-                                  bias.data_ptr() if bias is not None else None, 1 if activation == "relu" else 0, c.address, c_ld,
+        rc = L.dlf_b200_gemm_int8(prec, m, n, k, a, a_ld, a_scales, b, b_ld, b_scales, bias, activation, c, c_ld,
                                   ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, handle)
         if event is not None:
             event.end.record(s)
     _check(rc)
+
+
+class _Plans(dict):
+    """What is known of a call from its tensors' types, devices, shapes and strides - that they fit together, and the library's arguments
+    made of them - so that a call like an earlier one only looks this up. Started anew when it has grown."""
+
+    def keep(self, key, plan):
+        if len(self) >= 512:
+            self.clear()
+        self[key] = plan
+        return plan
 
 
 def gemmStridedBatched(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_offset, a_ld,

@@ -8,12 +8,13 @@ convolution's epilogue.
 """
 import ctypes
 import math
+import struct
 
 import torch
 
 from . import lib
-from .gblas import (BLASError, StatusCode, _NO_LOCK, _caller_scratch, _capturing, _check, _operator_scratch, _operator_stream,
-                    _passing_scratch, _ptr, _stream, _stream_scratch, precision_of)
+from .gblas import (BLASError, StatusCode, _NO_LOCK, _Plans, _caller_scratch, _capturing, _check, _operator_scratch,
+                    _operator_stream, _passing_scratch, _ptr, _stream, _stream_scratch, precision_of)
 
 
 class Filter2D:
@@ -320,27 +321,31 @@ def pool_nhwc(X, Y, filt, average=False, count_include_pad=False, queue=None):
 # products and a softmax between them.
 
 _ATTENTION_WORKSPACES = {}
-_THREE = ctypes.c_size_t * 3
-_INT8_TYPES = (torch.bool, torch.uint8)
+_MASK_TYPES = (torch.bool, torch.uint8)
+# the structures of the C header without their pointers, and the pointers
+_ATTENTION_ARGS, _PAGED_ARGS, _APPEND_ARGS = struct.Struct("@if19N"), struct.Struct("@if18N"), struct.Struct("@iN17N")
+_SIX_POINTERS, _SEVEN_POINTERS = struct.Struct("@6P"), struct.Struct("@7P")
 
 
-def _head_tensor(t, dtype, device, dims):
-    """Checks a tensor of heads; its strides without the last dimension's."""
-    if t.dtype != dtype:
-        raise BLASError(StatusCode.kInvalidValue)
-    if t.dim() != dims:
-        raise BLASError(StatusCode.kInvalidDimension)
-    if t.device != device:
-        raise BLASError(StatusCode.kInvalidMatrixA)
-    s = t.stride()
-    if s[-1] != 1 and t.shape[-1] != 1:
+_ATTENTION_PLANS, _PAGED_PLANS, _APPEND_PLANS = _Plans(), _Plans(), _Plans()
+
+
+def _head_strides(shape, strides):
+    """Strides of a tensor of heads for the library, without the last dimension's; where there is only one, 8 elements stand for
+    whatever is written."""
+    if strides[-1] != 1 and shape[-1] != 1:
         raise BLASError(StatusCode.kNotImplemented)
-    return s
+    return [s if n > 1 else 8 for n, s in zip(shape[:-1], strides)]
 
 
-def _strides(shape, strides):
-    """Strides for the library; where there is only one, 8 elements stand for whatever is written."""
-    return _THREE(*[s if n > 1 else 8 for n, s in zip(shape[:-1], strides)])
+def _same(tensors, dtype, device, dims):
+    for t in tensors:
+        if t.dtype != dtype:
+            raise BLASError(StatusCode.kInvalidValue)
+        if t.dim() != dims or 0 in t.shape:
+            raise BLASError(StatusCode.kInvalidDimension)
+        if t.device != device or device.type != "cuda":
+            raise BLASError(StatusCode.kInvalidMatrixA)
 
 
 def _device_ints(t, count, device):
@@ -360,8 +365,8 @@ def _default_scale(scale, size):
     return scale
 
 
-def _attention_call(need, device, queue, event, call):
-    """call(workspace, bytes, stream) with scratch of `need` bytes."""
+def _attention_call(fn, args, need, device, queue, event):
+    """fn(args, [workspace, bytes,] stream) with scratch of `need` bytes (None: fn takes none)."""
     handle = _operator_stream(queue, device)
     ws, entry = _operator_scratch(_ATTENTION_WORKSPACES, need, device, queue, handle) if need else (None, None)
     with entry.lock if entry is not None else _NO_LOCK:
@@ -370,10 +375,31 @@ def _attention_call(need, device, queue, event, call):
         if event is not None:
             s = queue if queue is not None else torch.cuda.current_stream()
             event.start.record(s)
-        rc = call(ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, handle)
+        if need is None:
+            rc = fn(args, handle)
+        else:
+            rc = fn(args, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0, handle)
         if event is not None:
             event.end.record(s)
     _check(rc)
+
+
+def _attention_plan(Q, K, V, Y, scale, key_mask):
+    _same((Q, K, V, Y), Y.dtype, Y.device, 4)
+    b, lq, h, d = Q.shape
+    lk, hk = K.shape[1:3]
+    if K.shape[0] != b or K.shape[3] != d or V.shape != K.shape or Y.shape != Q.shape or h % hk:
+        raise BLASError(StatusCode.kInvalidDimension)
+    mask_ld = 0
+    if key_mask is not None:
+        if key_mask.dtype not in _MASK_TYPES or tuple(key_mask.shape) != (b, lk) or (lk > 1 and key_mask.stride(1) != 1):
+            raise BLASError(StatusCode.kInvalidValue)
+        if key_mask.device != Y.device:
+            raise BLASError(StatusCode.kInvalidMatrixA)
+        mask_ld = key_mask.stride(0) if b > 1 else lk
+    strides = [s for t in (Q, K, V, Y) for s in _head_strides(t.shape, t.stride())]
+    args = _ATTENTION_ARGS.pack(int(precision_of(Y)), _default_scale(scale, d), b, lq, lk, h, hk, d, *strides, mask_ld)
+    return args, lib().dlf_b200_attention_workspace_bytes(b, lq, lk, h, hk, d), b, Y.device
 
 
 def attention(Q, K, V, Y, scale=None, key_lengths=None, key_mask=None, queue=None, event=None):
@@ -383,42 +409,44 @@ def attention(Q, K, V, Y, scale=None, key_lengths=None, key_mask=None, queue=Non
 
     ``key_lengths`` (batch, int32) and ``key_mask`` (batch, keys; bool or uint8, 0 = left out) say which keys count; those that do not
     may hold anything. A query with no key gets zeros. Any strides that are multiples of 8 elements, over 16-byte aligned
-    addresses, with a head's values contiguous; K and V may be shared by the batch (expanded)."""
-    device, dtype = Y.device, Y.dtype
-    prec = precision_of(Y)
-    qs, ks, vs, ys = (_head_tensor(t, dtype, device, 4) for t in (Q, K, V, Y))
-    b, lq, h, d = Q.shape
-    lk, hk = K.shape[1:3]
-    if K.shape[0] != b or K.shape[3] != d or V.shape != K.shape or Y.shape != Q.shape or 0 in Q.shape or 0 in K.shape or h % hk:
-        raise BLASError(StatusCode.kInvalidDimension)
-    scale = _default_scale(scale, d)
-    lengths = _device_ints(key_lengths, b, device) if key_lengths is not None else None
-    mask, mask_ld = None, 0
-    if key_mask is not None:
-        if key_mask.dtype not in _INT8_TYPES or tuple(key_mask.shape) != (b, lk) or (lk > 1 and key_mask.stride(1) != 1):
-            raise BLASError(StatusCode.kInvalidValue)
-        if key_mask.device != device:
-            raise BLASError(StatusCode.kInvalidMatrixA)
-        mask, mask_ld = key_mask.data_ptr(), key_mask.stride(0) if b > 1 else lk
-    if not Y.is_cuda:
-        raise BLASError(StatusCode.kInvalidMatrixA)
-    L = lib()
-    _attention_call(L.dlf_b200_attention_workspace_bytes(b, lq, lk, h, hk, d), device, queue, event,
-                    lambda ws, n, stream: L.dlf_b200_attention(
-                        int(prec), b, lq, lk, h, hk, d, scale, Q.data_ptr(), _strides(Q.shape, qs), K.data_ptr(), _strides(K.shape, ks),
-                        V.data_ptr(), _strides(V.shape, vs), lengths, mask, mask_ld, Y.data_ptr(), _strides(Y.shape, ys), ws, n, stream))
+    addresses, with a head's values contiguous; Q, K and V may be shared by the batch (expanded)."""
+    key = (Q.dtype, K.dtype, V.dtype, Y.dtype, Q.device, K.device, V.device, Y.device, Q.shape, K.shape, V.shape, Y.shape, Q.stride(), K.stride(),
+           V.stride(), Y.stride(), scale,
+           None if key_mask is None else (key_mask.dtype, key_mask.device, key_mask.shape, key_mask.stride()))
+    plan = _ATTENTION_PLANS.get(key)
+    if plan is None:
+        plan = _ATTENTION_PLANS.keep(key, _attention_plan(Q, K, V, Y, scale, key_mask))
+    args, need, batch, device = plan
+    pointers = _SIX_POINTERS.pack(Q.data_ptr(), K.data_ptr(), V.data_ptr(), Y.data_ptr(),
+                                  0 if key_lengths is None else _device_ints(key_lengths, batch, device),
+                                  0 if key_mask is None else key_mask.data_ptr())
+    _attention_call(lib().dlf_b200_attention, args + pointers, need, device, queue, event)
 
 
-def _cache_tensors(K_pages, V_pages, page_table, dtype, device):
-    ks, vs = (_head_tensor(t, dtype, device, 4) for t in (K_pages, V_pages))
-    if V_pages.shape != K_pages.shape or 0 in K_pages.shape or page_table.dim() != 2 or 0 in page_table.shape:
+def _table_plan(K_pages, V_pages, page_table):
+    """(strides of the cache's tensors, width and leading dimension of the page table)"""
+    if V_pages.shape != K_pages.shape or page_table.dim() != 2 or 0 in page_table.shape:
         raise BLASError(StatusCode.kInvalidDimension)
-    if page_table.dtype != torch.int32 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    n, width = page_table.shape
+    if page_table.dtype != torch.int32 or (width > 1 and page_table.stride(1) != 1):
         raise BLASError(StatusCode.kInvalidValue)
-    if page_table.device != device:
+    if page_table.device != K_pages.device:
         raise BLASError(StatusCode.kInvalidMatrixA)
-    width = page_table.shape[1]
-    return _strides(K_pages.shape, ks), _strides(V_pages.shape, vs), width, page_table.stride(0) if page_table.shape[0] > 1 else width
+    strides = [_head_strides(t.shape, t.stride()) for t in (K_pages, V_pages)]
+    return strides, width, page_table.stride(0) if n > 1 else width
+
+
+def _paged_plan(Q, K_pages, V_pages, page_table, Y, scale):
+    _same((Q, Y), Y.dtype, Y.device, 3)
+    _same((K_pages, V_pages), Y.dtype, Y.device, 4)
+    b, h, d = Q.shape
+    pages, page_size, hk, dk = K_pages.shape
+    (ks, vs), width, ld = _table_plan(K_pages, V_pages, page_table)
+    if dk != d or Y.shape != Q.shape or page_table.shape[0] != b or h % hk:
+        raise BLASError(StatusCode.kInvalidDimension)
+    args = _PAGED_ARGS.pack(int(precision_of(Y)), _default_scale(scale, d), b, h, hk, d, pages, page_size, width, ld,
+                            *_head_strides(Q.shape, Q.stride()), *ks, *vs, *_head_strides(Y.shape, Y.stride()))
+    return args, lib().dlf_b200_paged_attention_workspace_bytes(b, h, hk, d), b, Y.device
 
 
 def paged_attention(Q, K_pages, V_pages, page_table, lengths, Y, scale=None, queue=None, event=None):
@@ -426,41 +454,41 @@ def paged_attention(Q, K_pages, V_pages, page_table, lengths, Y, scale=None, que
     V_pages (pages, page_size, kv_heads, size; any strides as in ``attention``). Position i of sequence b lies in page
     page_table[b][i // page_size] (int32) at i % page_size; lengths[b] (int32) positions count, the new token's among them if
     ``paged_append`` has put it there. Table entries beyond a sequence's length may be anything."""
-    device, dtype = Y.device, Y.dtype
-    prec = precision_of(Y)
-    qs, ys = _head_tensor(Q, dtype, device, 3), _head_tensor(Y, dtype, device, 3)
-    b, h, d = Q.shape
-    kst, vst, width, ld = _cache_tensors(K_pages, V_pages, page_table, dtype, device)
-    pages, page_size, hk, dk = K_pages.shape
-    if dk != d or Y.shape != Q.shape or 0 in Q.shape or page_table.shape[0] != b or h % hk:
+    key = (Q.dtype, K_pages.dtype, V_pages.dtype, Y.dtype, page_table.dtype, Q.device, K_pages.device, V_pages.device, Y.device,
+           page_table.device, Q.shape, K_pages.shape, V_pages.shape, Y.shape, page_table.shape, Q.stride(), K_pages.stride(), V_pages.stride(),
+           Y.stride(), page_table.stride(), scale)
+    plan = _PAGED_PLANS.get(key)
+    if plan is None:
+        plan = _PAGED_PLANS.keep(key, _paged_plan(Q, K_pages, V_pages, page_table, Y, scale))
+    args, need, batch, device = plan
+    pointers = _SIX_POINTERS.pack(Q.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), Y.data_ptr(), page_table.data_ptr(),
+                                  _device_ints(lengths, batch, device))
+    _attention_call(lib().dlf_b200_paged_attention, args + pointers, need, device, queue, event)
+
+
+def _append_plan(K, V, K_pages, V_pages, page_table):
+    _same((K, V), K_pages.dtype, K_pages.device, 3)
+    _same((K_pages, V_pages), K_pages.dtype, K_pages.device, 4)
+    pages, page_size, hk, d = K_pages.shape
+    (ks, vs), width, ld = _table_plan(K_pages, V_pages, page_table)
+    if K.shape != V.shape or tuple(K.shape[1:]) != (hk, d):
         raise BLASError(StatusCode.kInvalidDimension)
-    scale = _default_scale(scale, d)
-    n = _device_ints(lengths, b, device)
-    if not Y.is_cuda:
-        raise BLASError(StatusCode.kInvalidMatrixA)
-    L = lib()
-    _attention_call(L.dlf_b200_paged_attention_workspace_bytes(b, h, hk, d), device, queue, event,
-                    lambda ws, nbytes, stream: L.dlf_b200_paged_attention(
-                        int(prec), b, h, hk, d, scale, Q.data_ptr(), _strides(Q.shape, qs), K_pages.data_ptr(), kst, V_pages.data_ptr(), vst,
-                        pages, page_size, page_table.data_ptr(), width, ld, n, Y.data_ptr(), _strides(Y.shape, ys), ws, nbytes, stream))
+    args = _APPEND_ARGS.pack(int(precision_of(K_pages)), K.shape[0], hk, d, page_table.shape[0], pages, page_size, width, ld,
+                             *_head_strides(K.shape, K.stride()), *_head_strides(V.shape, V.stride()), *ks, *vs)
+    return args, K.shape[0], K_pages.device
 
 
 def paged_append(K, V, K_pages, V_pages, page_table, positions, sequences=None, queue=None, event=None):
     """New keys and values K and V (tokens, kv_heads, size) into a paged cache (see ``paged_attention``): token i to position
     positions[i] of sequence sequences[i] (both int32; without ``sequences``, of sequence i). The rest of the cache stays as it is."""
-    device, dtype = K_pages.device, K_pages.dtype
-    prec = precision_of(K_pages)
-    kns, vns = _head_tensor(K, dtype, device, 3), _head_tensor(V, dtype, device, 3)
-    kst, vst, width, ld = _cache_tensors(K_pages, V_pages, page_table, dtype, device)
-    pages, page_size, hk, d = K_pages.shape
-    t = K.shape[0]
-    if K.shape != V.shape or tuple(K.shape[1:]) != (hk, d) or t == 0 or (sequences is None and t > page_table.shape[0]):
-        raise BLASError(StatusCode.kInvalidDimension)
-    pos = _device_ints(positions, t, device)
-    seq = _device_ints(sequences, t, device) if sequences is not None else None
-    if not K_pages.is_cuda:
-        raise BLASError(StatusCode.kInvalidMatrixA)
-    _attention_call(0, device, queue, event,
-                    lambda ws, n, stream: lib().dlf_b200_paged_append(
-                        int(prec), t, hk, d, K.data_ptr(), _strides(K.shape, kns), V.data_ptr(), _strides(V.shape, vns), K_pages.data_ptr(), kst,
-                        V_pages.data_ptr(), vst, pages, page_size, page_table.data_ptr(), page_table.shape[0], width, ld, pos, seq, stream))
+    key = (K.dtype, V.dtype, K_pages.dtype, V_pages.dtype, page_table.dtype, K.device, V.device, K_pages.device, V_pages.device,
+           page_table.device, K.shape, V.shape, K_pages.shape, V_pages.shape, page_table.shape, K.stride(), V.stride(), K_pages.stride(),
+           V_pages.stride(), page_table.stride())
+    plan = _APPEND_PLANS.get(key)
+    if plan is None:
+        plan = _APPEND_PLANS.keep(key, _append_plan(K, V, K_pages, V_pages, page_table))
+    args, tokens, device = plan
+    pointers = _SEVEN_POINTERS.pack(K.data_ptr(), V.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), page_table.data_ptr(),
+                                    _device_ints(positions, tokens, device),
+                                    0 if sequences is None else _device_ints(sequences, tokens, device))
+    _attention_call(lib().dlf_b200_paged_append, args + pointers, None, device, queue, event)

@@ -253,8 +253,11 @@ def matmul(A, B, C=None, alpha=1, beta=0, backend=None, trace=None):
     return C
 
 
+_QUANTIZE_PLANS, _INT8_PLANS = _gblas._Plans(), _gblas._Plans()
+
+
 def _rows(t, what):
-    """A (..., n) tensor as a matrix of its rows: (matrix, rows, n, elements between rows)."""
+    """A (..., n) tensor as a matrix of its rows: (rows, n, elements between rows)."""
     if t.dim() != 2:
         try:
             t = t.view(-1, t.shape[-1])
@@ -262,12 +265,33 @@ def _rows(t, what):
             raise ShapeError("%s: the rows must be evenly spaced" % what)
     m, n = t.shape
     ld, inc = t.stride()
+    if m == 0 or n == 0:
+        raise _gblas.BLASError(_gblas.StatusCode.kInvalidDimension)
     if inc != 1 and n > 1:
         raise ShapeError("%s: rows must be contiguous" % what)
-    return t, m, n, ld if m > 1 else max(ld, n)
+    return m, n, ld if m > 1 else max(ld, n)
 
 
-def quantize(X, Q=None, scales=None):
+def _typed(what, device, *tensors):
+    for t, dtype in tensors:
+        if t.dtype != dtype:
+            raise _gblas.BLASError(_gblas.StatusCode.kInvalidValue)
+        if t.device != device or device.type != "cuda":
+            raise _gblas.BLASError(_gblas.StatusCode.kInvalidMatrixA)
+
+
+def _quantize_plan(X, Q, scales):
+    if Q.shape != X.shape:
+        raise ShapeError("quantize: Q must have the shape of X")
+    if scales.shape != X.shape[:-1] or not scales.is_contiguous():
+        raise ShapeError("quantize: one scale for each row of X, contiguous")
+    prec = _gblas.precision_of(X)
+    _typed("quantize", X.device, (X, X.dtype), (Q, torch.int8), (scales, torch.float32))
+    m, n, x_ld = _rows(X, "quantize")
+    return int(prec), m, n, x_ld, _rows(Q, "quantize")[2], X.device
+
+
+def quantize(X, Q=None, scales=None, queue=None, event=None):
     """The rows of X (..., n) as 8-bit integers Q (..., n) and fp32 scales (...): row = Q * scale, to within half a scale
     (``gblas.quantizeRows``). Returns (Q, scales). A Q allocated here has rows on 16-byte boundaries, the form that
     ``matmul_int8`` reads without a copy."""
@@ -276,42 +300,54 @@ def quantize(X, Q=None, scales=None):
     if Q is None:
         n = X.shape[-1]
         Q = torch.empty(X.shape[:-1] + ((n + 15) // 16 * 16,), dtype=torch.int8, device=X.device)[..., :n]
-    elif Q.shape != X.shape:
-        raise ShapeError("quantize: Q must have the shape of X")
     if scales is None:
         scales = torch.empty(X.shape[:-1], dtype=torch.float32, device=X.device)
-    elif scales.shape != X.shape[:-1]:
-        raise ShapeError("quantize: one scale for each row of X")
-    if not scales.is_contiguous():
-        raise ShapeError("quantize: the scales must be contiguous")
-    x, m, n, x_ld = _rows(X, "quantize")
-    q, _, _, q_ld = _rows(Q, "quantize")
-    _gblas._quantize_rows(m, n, _gblas._view_operand(x), x_ld, _gblas._view_operand(q), q_ld, scales)
+    key = (X.dtype, Q.dtype, scales.dtype, X.device, Q.device, scales.device, X.shape, Q.shape, scales.shape, X.stride(), Q.stride(),
+           scales.stride())
+    plan = _QUANTIZE_PLANS.get(key)
+    if plan is None:
+        plan = _QUANTIZE_PLANS.keep(key, _quantize_plan(X, Q, scales))
+    prec, m, n, x_ld, q_ld, device = plan
+    _gblas._quantize_rows(prec, m, n, X.data_ptr(), x_ld, Q.data_ptr(), q_ld, scales.data_ptr(), device, queue, event)
     return Q, scales
 
 
-def matmul_int8(A, a_scales, B, b_scales, C=None, bias=None, activation=None, dtype=torch.float32):
-    """C = act((A @ B^T) * a_scales * b_scales + bias) for 8-bit integers A (..., k) with a scale for each row (token) and B (n, k)
-    with one for each of its rows (output channel): a quantised layer (``gblas.gemmInt8``). C (..., n) is allocated with
-    ``dtype`` when not given."""
+def _int8_plan(A, a_scales, B, b_scales, C, bias, activation):
     if A.dim() < 1 or B.dim() != 2:
         raise ShapeError("matmul_int8: A must have rows and B must be a matrix")
     if A.shape[-1] != B.shape[1]:
         raise ShapeError("matmul_int8: incompatible shape")
-    if a_scales.shape != A.shape[:-1] or tuple(b_scales.shape) != (B.shape[0],):
-        raise ShapeError("matmul_int8: one scale for each row of A and of B")
-    shape = A.shape[:-1] + (B.shape[0],)
-    if C is None:
-        C = torch.empty(shape, dtype=dtype, device=A.device)
-    elif C.shape != shape:
+    if a_scales.shape != A.shape[:-1] or tuple(b_scales.shape) != (B.shape[0],) or not (a_scales.is_contiguous() and b_scales.is_contiguous()):
+        raise ShapeError("matmul_int8: one scale for each row of A and of B, contiguous")
+    if C.shape != A.shape[:-1] + (B.shape[0],):
         raise ShapeError("matmul_int8: bad output shape")
-    if bias is not None and tuple(bias.shape) != (B.shape[0],):
-        raise ShapeError("matmul_int8: one bias for each row of B")
-    a, m, k, a_ld = _rows(A, "matmul_int8")
-    b, n, _, b_ld = _rows(B, "matmul_int8")
-    c, _, _, c_ld = _rows(C, "matmul_int8")
-    v = _gblas._view_operand
-    _gblas._gemm_int8(m, n, k, v(a), a_ld, a_scales, v(b), b_ld, b_scales, v(c), c_ld, bias, activation)
+    if bias is not None and (tuple(bias.shape) != (B.shape[0],) or not bias.is_contiguous()):
+        raise ShapeError("matmul_int8: one bias for each row of B, contiguous")
+    if activation not in (None, "relu"):
+        raise _gblas.BLASError(_gblas.StatusCode.kInvalidValue)
+    prec = _gblas.precision_of(C)
+    _typed("matmul_int8", C.device, (C, C.dtype), (A, torch.int8), (B, torch.int8), (a_scales, torch.float32), (b_scales, torch.float32),
+           *([(bias, C.dtype)] if bias is not None else []))
+    m, k, a_ld = _rows(A, "matmul_int8")
+    n, _, b_ld = _rows(B, "matmul_int8")
+    return int(prec), m, n, k, a_ld, b_ld, 1 if activation == "relu" else 0, _rows(C, "matmul_int8")[2], C.device
+
+
+def matmul_int8(A, a_scales, B, b_scales, C=None, bias=None, activation=None, dtype=torch.float32, queue=None, event=None):
+    """C = act((A @ B^T) * a_scales * b_scales + bias) for 8-bit integers A (..., k) with a scale for each row (token) and B (n, k)
+    with one for each of its rows (output channel): a quantised layer (``gblas.gemmInt8``). C (..., n) is allocated with
+    ``dtype`` when not given. Rows of A and B that lie on 16-byte boundaries are read as they are, others are copied first."""
+    if C is None:
+        C = torch.empty(A.shape[:-1] + B.shape[:1], dtype=dtype, device=A.device)
+    key = (A.dtype, B.dtype, C.dtype, a_scales.dtype, b_scales.dtype, A.device, B.device, C.device, a_scales.device, b_scales.device, A.shape,
+           B.shape, C.shape, a_scales.shape, b_scales.shape, A.stride(), B.stride(), C.stride(), a_scales.stride(), b_scales.stride(), activation,
+           None if bias is None else (bias.dtype, bias.device, bias.shape, bias.stride()))
+    plan = _INT8_PLANS.get(key)
+    if plan is None:
+        plan = _INT8_PLANS.keep(key, _int8_plan(A, a_scales, B, b_scales, C, bias, activation))
+    prec, m, n, k, a_ld, b_ld, act, c_ld, device = plan
+    _gblas._gemm_int8(prec, m, n, k, A.data_ptr(), a_ld, a_scales.data_ptr(), B.data_ptr(), b_ld, b_scales.data_ptr(),
+                      bias.data_ptr() if bias is not None else None, act, C.data_ptr(), c_ld, device, queue, event)
     return C
 
 

@@ -296,21 +296,41 @@ size_t dlf_b200_gemm_int8_workspace_bytes(size_t m, size_t n, size_t k, const si
  * Lengths below 0 count as 0 and those beyond the keys there are as all of them; keys on a page that is none of the
  * num_pages do not count, and tokens for a position or page that does not exist are left out. Such lengths, positions and pages are
  * reported by bit 1 of dlf_b200_device_status (a length below 0 is not); nothing outside the tensors is read or written. */
+typedef struct {
+    int dtype;
+    float scale;
+    size_t batch, queries, keys, heads, kv_heads, size;
+    size_t q_strides[3], k_strides[3], v_strides[3], y_strides[3];
+    size_t key_mask_ld;
+    const void *q, *k, *v;
+    void* y;
+    const int* key_lengths;
+    const unsigned char* key_mask;
+} dlf_b200_attention_args;
 size_t dlf_b200_attention_workspace_bytes(size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size);
-int dlf_b200_attention(int dtype, size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size, float scale,
-                       const void* q, const size_t* q_strides, const void* k, const size_t* k_strides, const void* v,
-                       const size_t* v_strides, const int* key_lengths, const unsigned char* key_mask, size_t key_mask_ld, void* y,
-                       const size_t* y_strides, void* workspace, size_t workspace_bytes, void* stream);
+int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct {
+    int dtype;
+    float scale;
+    size_t batch, heads, kv_heads, size, num_pages, page_size, table_width, table_ld;
+    size_t q_strides[2], k_strides[3], v_strides[3], y_strides[2];
+    const void *q, *k_pages, *v_pages;
+    void* y;
+    const int *page_table, *lengths;
+} dlf_b200_paged_attention_args;
 size_t dlf_b200_paged_attention_workspace_bytes(size_t batch, size_t heads, size_t kv_heads, size_t size);
-int dlf_b200_paged_attention(int dtype, size_t batch, size_t heads, size_t kv_heads, size_t size, float scale, const void* q,
-                             const size_t* q_strides, const void* k_pages, const size_t* k_strides, const void* v_pages,
-                             const size_t* v_strides, size_t num_pages, size_t page_size, const int* page_table, size_t table_width,
-                             size_t table_ld, const int* lengths, void* y, const size_t* y_strides, void* workspace,
-                             size_t workspace_bytes, void* stream);
-int dlf_b200_paged_append(int dtype, size_t tokens, size_t kv_heads, size_t size, const void* k, const size_t* k_strides, const void* v,
-                          const size_t* v_strides, void* k_pages, const size_t* kp_strides, void* v_pages, const size_t* vp_strides,
-                          size_t num_pages, size_t page_size, const int* page_table, size_t batch, size_t table_width,
-                          size_t table_ld, const int* positions, const int* sequences, void* stream);
+int dlf_b200_paged_attention(const dlf_b200_paged_attention_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct {
+    int dtype;
+    size_t tokens, kv_heads, size, batch, num_pages, page_size, table_width, table_ld; /* batch: lines of the page table */
+    size_t k_strides[2], v_strides[2], k_pages_strides[3], v_pages_strides[3];
+    const void *k, *v;
+    void *k_pages, *v_pages;
+    const int *page_table, *positions, *sequences;
+} dlf_b200_paged_append_args;
+int dlf_b200_paged_append(const dlf_b200_paged_append_args* args, void* stream);
 
 /* Name of a status code returned by the functions above (static storage). Mirrors the
  * StatusCode enumerators of gblas.h:43-107. */
