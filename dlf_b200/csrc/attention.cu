@@ -57,6 +57,8 @@ bool strides_ok(std::initializer_list<size_t> s) {
     return true;
 }
 
+// (sequences of one tile of keys are never cut)
+size_t tiles_workspace(size_t keys, size_t size) { return keys > kTileKeys ? static_cast<size_t>(2 * kB200Sms) * tiles_slot(static_cast<int>(size)) * 4 : 0; }
 size_t decode_workspace(size_t size) { return static_cast<size_t>(2 * kB200Sms * decode_ctas_per_sm(static_cast<int>(size), 1)) * decode_slot(static_cast<int>(size)) * 4; }
 
 template <bool BF16, int DP, int KEYS, int NB, bool FULL>
@@ -89,24 +91,36 @@ int decode_any(DecodeParams& p, bool bf16, cudaStream_t stream) {
     return bf16 ? decode_rows<true, 128>(p, stream) : decode_rows<false, 128>(p, stream);
 }
 
-// tensor map of a (batch, tokens, heads, size) tensor: boxes of `rows` tokens x 64 values of one head, 128-byte swizzle
+// tensor map of a (batch, tokens, heads, size) tensor: boxes of `rows` tokens x 64 (or 32) values of one head, swizzled by 128 (64) bytes
 int encode_heads(const OperatorDevice& dev, CUtensorMap* map, const void* base, size_t size, size_t tokens, size_t heads, size_t batch,
-                 size_t st, size_t sh, size_t sb, unsigned rows) {
+                 size_t st, size_t sh, size_t sb, unsigned rows, unsigned values = 64) {
     auto stride = [](size_t extent, size_t s) { return static_cast<cuuint64_t>(extent > 1 && s > 0 ? s * 2 : 16); };
     cuuint64_t dims[4] = {size, tokens, heads, sb == 0 ? 1 : batch};
     cuuint64_t strides[3] = {stride(tokens, st), stride(heads, sh), stride(dims[3], sb)};
-    cuuint32_t box[4] = {64, rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+    cuuint32_t box[4] = {values, rows, 1, 1}, estr[4] = {1, 1, 1, 1};
     const CUresult r = dev.encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides, box, estr,
-                                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                  CU_TENSOR_MAP_INTERLEAVE_NONE, values == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? kSuccess : kUnexpectedError;
 }
 
 template <bool BF16, int DP>
-int tiles_launch(const TilesParams& p, unsigned grid, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& y,
-                 cudaStream_t stream) {
-    CUDA_TRY(launch_dependent(attention_tiles_kernel<BF16, DP>, grid, kTilesThreads, tiles_smem(DP), stream, p, q, k, v, y));
+int tiles_launch(const TilesParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& y, cudaStream_t stream) {
+    CUDA_TRY(launch_dependent(attention_tiles_kernel<BF16, DP>, static_cast<unsigned>(p.ctas), kTilesThreads, tiles_smem(DP), stream, p, q, k, v, y));
     count_launch();
+    if (p.keys > kTileKeys && p.ctas > 1) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(p.ctas - 1), 256 / kTilesJoinRows, 1);
+        cfg.blockDim = dim3(128, 1, 1);
+        cfg.stream = stream;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr.val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        CUDA_TRY(cudaLaunchKernelEx(&cfg, attention_tiles_join_kernel<BF16>, p));
+        count_launch();
+    }
     CUDA_TRY(cudaGetLastError());
     return kSuccess;
 }
@@ -127,9 +141,8 @@ extern "C" {
 
 size_t dlf_b200_attention_workspace_bytes(size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size) {
     (void)batch;
-    (void)keys;
     if (kv_heads == 0 || heads % kv_heads != 0) return 0;
-    return few_rows(queries, heads / kv_heads) ? decode_workspace(size) : 0;
+    return few_rows(queries, heads / kv_heads) ? decode_workspace(size) : tiles_workspace(keys, size);
 }
 
 int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -154,10 +167,10 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     const bool bf16 = dtype == DLF_B200_BFLOAT16;
     const size_t group = heads / kv_heads;
     const bool few = few_rows(queries, group);
-    if (few && (workspace == nullptr || workspace_bytes < dlf_b200_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, size)))
-        return kInsufficientMemoryTemp;
+    const size_t need = dlf_b200_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, size);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return kInsufficientMemoryTemp;
     const long long items = static_cast<long long>((queries + 255) / 256) * static_cast<long long>(heads) * static_cast<long long>(batch);
-    if (items > INT_MAX / 2 || static_cast<double>(batch) * heads * (keys / kPlanUnit + 1.0) > 2147483647.0) return kInvalidDimension;
+    if (static_cast<double>(items) * (static_cast<double>(keys) / kTileKeys + 1.0) > 2147483647.0 || static_cast<double>(batch) * heads * (keys / kDecodeUnit + 1.0) > 2147483647.0) return kInvalidDimension;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     StreamDevice guard(s);
     if (guard.rc != kSuccess) return guard.rc;
@@ -200,31 +213,33 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     p.queries = static_cast<int>(queries);
     p.keys = static_cast<int>(keys);
     p.heads = static_cast<int>(heads);
-    p.kv_heads = static_cast<int>(kv_heads);
     p.group = static_cast<int>(group);
     p.size = static_cast<int>(size);
     p.lengths = key_lengths;
     p.mask = key_mask;
     p.mask_sb = static_cast<long long>(key_mask_ld);
     p.q_pairs = static_cast<int>((queries + 255) / 256);
-    p.items = static_cast<int>(items);
+    const long long units = items * static_cast<long long>((keys + kTileKeys - 1) / kTileKeys);
+    p.ctas = static_cast<int>(std::min<long long>(units, std::min(dev.num_sms, kB200Sms)));
+    p.y = static_cast<char*>(y);
+    p.y_sb = y_strides[0], p.y_st = y_strides[1], p.y_sh = y_strides[2];
+    p.parts = static_cast<float*>(workspace);
     p.q_batched = q_strides[0] != 0;
     p.k_batched = k_strides[0] != 0;
     p.v_batched = v_strides[0] != 0;
     p.c = c;
     p.status = dev.status;
-    const bool inject = (tuning_bits() & 0x10000000u) != 0 && p.items == 1;
+    const bool inject = (tuning_bits() & 0x10000000u) != 0 && units == 1;
     p.wait_limit = inject ? (1ll << 21) : (1ll << 32);
     p.withhold = inject ? 1 : 0;
     CUtensorMap mq, mk, mv, my;
     rc = encode_heads(dev, &mq, q, size, queries, heads, batch, q_strides[1], q_strides[2], q_strides[0], 128);
     if (rc == kSuccess) rc = encode_heads(dev, &mk, k, size, keys, kv_heads, batch, k_strides[1], k_strides[2], k_strides[0], 128);
     if (rc == kSuccess) rc = encode_heads(dev, &mv, v, size, keys, kv_heads, batch, v_strides[1], v_strides[2], v_strides[0], 128);
-    if (rc == kSuccess) rc = encode_heads(dev, &my, y, size, queries, heads, batch, y_strides[1], y_strides[2], y_strides[0], 32);
+    if (rc == kSuccess) rc = encode_heads(dev, &my, y, size, queries, heads, batch, y_strides[1], y_strides[2], y_strides[0], 32, size <= 64 ? 32 : 64);
     if (rc != kSuccess) return rc;
-    const unsigned grid = static_cast<unsigned>(std::min<long long>(items, dev.num_sms));
-    if (size <= 64) return bf16 ? tiles_launch<true, 64>(p, grid, mq, mk, mv, my, s) : tiles_launch<false, 64>(p, grid, mq, mk, mv, my, s);
-    return bf16 ? tiles_launch<true, 128>(p, grid, mq, mk, mv, my, s) : tiles_launch<false, 128>(p, grid, mq, mk, mv, my, s);
+    if (size <= 64) return bf16 ? tiles_launch<true, 64>(p, mq, mk, mv, my, s) : tiles_launch<false, 64>(p, mq, mk, mv, my, s);
+    return bf16 ? tiles_launch<true, 128>(p, mq, mk, mv, my, s) : tiles_launch<false, 128>(p, mq, mk, mv, my, s);
 }
 
 size_t dlf_b200_paged_attention_workspace_bytes(size_t batch, size_t heads, size_t kv_heads, size_t size) {
@@ -254,7 +269,7 @@ int dlf_b200_paged_attention(const dlf_b200_paged_attention_args* args, void* wo
                      y_strides[1]}))
         return kNotImplemented;
     if ((batch > 1 && y_strides[0] == 0) || (heads > 1 && y_strides[1] == 0)) return kInvalidLeadDimC;
-    if (static_cast<double>(batch) * heads * (static_cast<double>(table_width) * page_size / kPlanUnit + 1.0) > 2147483647.0) return kInvalidDimension;
+    if (static_cast<double>(batch) * heads * (static_cast<double>(table_width) * page_size / kDecodeUnit + 1.0) > 2147483647.0) return kInvalidDimension;
     if (workspace == nullptr || workspace_bytes < dlf_b200_paged_attention_workspace_bytes(batch, heads, kv_heads, size)) return kInsufficientMemoryTemp;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     StreamDevice guard(s);

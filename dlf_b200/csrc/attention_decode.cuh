@@ -26,8 +26,6 @@
 
 namespace dlfb200 {
 
-enum : int { DEV_STATUS_BAD_PAGE = 2 };  // (bit 1 of the status word) a page table entry or a length beyond the cache
-
 struct DecodeParams {
     const char* q;  // (batch, tokens, heads, size)
     const char* k;
@@ -53,6 +51,7 @@ struct DecodeParams {
 // pages of any size, or under a mask (every key by itself)
 enum : int { KEYS_PLAIN = 0, KEYS_PAGES_16 = 1, KEYS_ANY = 2 };
 
+constexpr int kDecodeUnit = 64;  // keys
 constexpr int kDecodeThreads = 128;
 constexpr int kDecodeWarps = kDecodeThreads / 32;
 // Stages of a warp's ring and blocks of an SM: nb = 1 or 2 sets of eight query rows. More blocks with shorter rings carry short
@@ -122,65 +121,7 @@ __device__ __forceinline__ float2 unpack_16(uint32_t w) {
     else return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// length of sequence b's keys; warp-uniform
-__device__ __forceinline__ int decode_length(const DecodeParams& p, int b) {
-    if (p.lengths == nullptr) return p.keys;
-    bool bad = false;
-    const int n = plan_length(p.lengths[b], p.keys, &bad);
-    if (bad && threadIdx.x == 0) atomicOr(p.status, DEV_STATUS_BAD_PAGE);
-    return n;
-}
-
-// units of all sequences for one (kv head, row block), and of those before sequence `upto`; by one warp
-__device__ __forceinline__ void decode_units(const DecodeParams& p, int upto, long long& before, long long& all) {
-    if (p.lengths == nullptr) {
-        before = static_cast<long long>(upto) * plan_units(p.keys);
-        all = static_cast<long long>(p.batch) * plan_units(p.keys);
-        return;
-    }
-    const int lane = threadIdx.x & 31;
-    int lo = 0, sum = 0;  // (host: all units fit in 31 bits)
-    bool bad = false;
-    for (int b = lane; b < p.batch; b += 32) {
-        const int n = plan_units(plan_length(p.lengths[b], p.keys, &bad));
-        sum += n;
-        if (b < upto) lo += n;
-    }
-    before = __reduce_add_sync(0xffffffffu, lo);
-    all = __reduce_add_sync(0xffffffffu, sum);
-}
-
-// the sequence that unit u of the call (u < all * heads) belongs to, and how many units lie before that sequence
-__device__ __forceinline__ int decode_find(const DecodeParams& p, long long u, int heads, long long& before) {
-    if (p.lengths == nullptr) {
-        const long long n = static_cast<long long>(plan_units(p.keys)) * heads;
-        const int b = static_cast<int>(u / n);
-        before = b * n;
-        return b;
-    }
-    const int lane = threadIdx.x & 31;
-    long long sum = 0;
-    bool bad = false;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int b = b0 + lane;
-        const int n = b < p.batch ? plan_units(plan_length(p.lengths[b], p.keys, &bad)) : 0;
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const int x = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += x;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, b < p.batch && u < (sum + incl) * heads);
-        if (past) {
-            const int src = __ffs(past) - 1;
-            before = (sum + __shfl_sync(0xffffffffu, incl - n, src)) * heads;
-            return b0 + src;
-        }
-        sum += __shfl_sync(0xffffffffu, incl, 31);
-    }
-    before = sum * heads;
-    return p.batch;
-}
+__device__ __forceinline__ PlanLengths decode_lengths(const DecodeParams& p) { return PlanLengths{p.lengths, p.keys, p.batch, kDecodeUnit, p.status}; }
 
 template <bool BF16, int DP, int KEYS, int NB, bool FULL>  // FULL: the head has all DP values
 __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) attention_decode_kernel(const __grid_constant__ DecodeParams p) {
@@ -200,39 +141,26 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
     ptx::wait_for_dependencies();
     ptx::launch_dependents();  // (behind the wait: what runs before this kernel is done when the joining one starts)
 
-    const int heads = p.kv_heads * p.row_blocks;
-    long long before, all;
-    decode_units(p, 0, before, all);
-    all *= heads;
-    const long long per = plan_per(all, p.ctas, p.least);
-    long long u = blockIdx.x * per;
-    const long long end = min(u + per, all);
-    if (u >= end) return;
-    int b = decode_find(p, u, heads, before);
-    int len = decode_length(p, b);
-    int units = plan_units(len);
-    int hb = static_cast<int>((u - before) / units);       // head and row block
-    int unit0 = static_cast<int>(u - before - static_cast<long long>(hb) * units);
+    PlanWalk walk(decode_lengths(p), p.kv_heads * p.row_blocks, p.ctas, p.least);
     const int chunks = p.size / 8;
     const float c = p.c, limit = 8.0f / c;
     bool bad_page = false;
 
-    while (u < end) {
-        const int n_units = static_cast<int>(min(static_cast<long long>(units - unit0), end - u));
-        const bool whole = n_units == units;
-        const int slot = plan_slot(u, per);
-        const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * p.block_rows;
+    for (; walk.more(); walk.next()) {
+        const int n_units = walk.count(), b = walk.b, len = walk.len, unit0 = walk.unit0;
+        const bool whole = walk.whole();
+        const int hk = walk.head / p.row_blocks, row0 = (walk.head - hk * p.row_blocks) * p.block_rows;
         const int rows = min(8 * NB, p.tokens * p.group - row0);
         // ---------------------------------------------------------------- copies
         // step i of this warp: keys first_key + 64 i .. + 15
-        const int first_key = unit0 * kPlanUnit + warp * 16;
+        const int first_key = unit0 * kDecodeUnit + warp * 16;
         const long long kst = p.k_st * 2, vst = p.v_st * 2;  // bytes between tokens
         const char* kbase = p.k + (p.table != nullptr ? 0 : b * p.k_sb * 2) + hk * p.k_sh * 2 + t * 16;
         const char* vbase = p.v + (p.table != nullptr ? 0 : b * p.v_sb * 2) + hk * p.v_sh * 2 + vch * 16;
         // what a step needs to know before it can be fetched: KEYS_PAGES_16 its page, KEYS_ANY lane l < 16 the place of key l (-1: not
         // kept). Asked for a step ahead of the fetch.
         auto ask = [&](int i) -> long long {
-            const int pos = first_key + i * kPlanUnit + (KEYS == KEYS_ANY ? (lane & 15) : 0);
+            const int pos = first_key + i * kDecodeUnit + (KEYS == KEYS_ANY ? (lane & 15) : 0);
             if (KEYS == KEYS_PLAIN || i >= n_units || pos >= len) return -1;
             if (KEYS == KEYS_PAGES_16 || p.table != nullptr) {
                 const int pg = pos / p.page_size;
@@ -246,7 +174,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
         auto fetch = [&](int stage, int i, long long at) -> unsigned {
             const uint32_t kdst = ring + stage * STAGE + lane * 16;
             const uint32_t vdst = ring + stage * STAGE + VOFF + vkey * LINE;
-            const int left = len - (first_key + i * kPlanUnit);
+            const int left = len - (first_key + i * kDecodeUnit);
             if constexpr (KEYS != KEYS_ANY) {
                 const char* kp = kbase + g * kst;
                 const char* vp = vbase + vkey * vst;
@@ -254,8 +182,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
                     kp += ((at >> 32) * p.k_sb + static_cast<int>(at) * p.k_st) * 2;
                     vp += ((at >> 32) * p.v_sb + static_cast<int>(at) * p.v_st) * 2;
                 } else {
-                    kp += (first_key + static_cast<long long>(i) * kPlanUnit) * kst;
-                    vp += (first_key + static_cast<long long>(i) * kPlanUnit) * vst;
+                    kp += (first_key + static_cast<long long>(i) * kDecodeUnit) * kst;
+                    vp += (first_key + static_cast<long long>(i) * kDecodeUnit) * vst;
                 }
                 if (FULL && left >= 16 && (KEYS == KEYS_PLAIN || at >= 0)) {
 #pragma unroll
@@ -462,7 +390,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
                 }
             }
         __syncthreads();
-        float* part = p.parts + static_cast<long long>(slot) * decode_slot(p.size);
+        float* part = p.parts + static_cast<long long>(walk.slot()) * decode_slot(p.size);
         for (int id = threadIdx.x; id < rows * chunks; id += kDecodeThreads) {
             const int r = id / chunks, ch = id - r * chunks;
             float mm = -INFINITY, ll = 0.0f, f[kDecodeWarps], acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -496,15 +424,6 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
             }
         }
         __syncthreads();  // before the rings are filled again
-        // ---------------------------------------------------------------- next segment
-        u += n_units;
-        unit0 = 0;
-        if (u < end && ++hb == heads) {
-            hb = 0;
-            ++b;
-            len = decode_length(p, b);
-            units = plan_units(len);
-        }
     }
     if (bad_page) atomicOr(p.status, DEV_STATUS_BAD_PAGE);
 }
@@ -515,12 +434,12 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     const int heads = p.kv_heads * p.row_blocks;
     const int b = blockIdx.x / heads, hb = blockIdx.x - b * heads;
     // the lengths are those the kernel before this one has read, which it lets this one start behind
-    long long before, all;
-    decode_units(p, b, before, all);
-    const long long per = plan_per(all * heads, p.ctas, p.least);
-    const int units = plan_units(decode_length(p, b));
-    const long long first = before * heads + static_cast<long long>(hb) * units, last = first + units - 1;
-    const int c0 = static_cast<int>(first / per), c1 = static_cast<int>(last / per);
+    int before, all;
+    plan_sums(decode_lengths(p), b, before, all);
+    const int per = plan_per(all * heads, p.ctas, p.least);
+    const int units = plan_units(plan_sequence(decode_lengths(p), b), kDecodeUnit);
+    const int first = before * heads + hb * units, last = first + units - 1;
+    const int c0 = first / per, c1 = last / per;
     const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * p.block_rows;
     const int rows = min(p.block_rows, p.tokens * p.group - row0), chunks = p.size / 4;
     ptx::wait_for_dependencies();
