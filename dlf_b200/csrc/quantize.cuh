@@ -15,6 +15,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "pairs.cuh"
 #include "ptx.cuh"
 
 namespace dlfb200 {
@@ -116,22 +117,29 @@ __device__ __forceinline__ int quantize_one(float x, float s, float inv) {
 template <typename T>
 __device__ __forceinline__ uint2 quantize_piece(const QuantizePiece<T>& p, float s, float inv) {
     constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the rounded value
-    float m[8], off = 0.0f;
+    const uint64_t inv2 = ptx::pair_of(inv, inv), up = ptx::pair_of(kMagic, kMagic), down = ptx::pair_of(-kMagic, -kMagic);
+    const uint64_t minus = ptx::pair_of(-1.0f, -1.0f);
+    uint32_t m[8];
+    float off = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float t = p.value(i) * inv;
-        m[i] = t + kMagic;
-        off = fmaxf(off, fabsf(t - (m[i] - kMagic)));
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t t = ptx::mul_pair(ptx::pair_of(p.value(i), p.value(i + 1)), inv2);
+        const uint64_t r = ptx::add_pair(t, up);
+        float a, b;
+        ptx::of_pair(r, a, b);
+        m[i] = __float_as_uint(a);
+        m[i + 1] = __float_as_uint(b);
+        ptx::of_pair(ptx::fma_pair(ptx::add_pair(r, down), minus, t), a, b);
+        off = fmaxf(off, fabsf(a));
+        off = fmaxf(off, fabsf(b));
     }
     if (off > 0.5f - 0x1p-15f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m[i] = kMagic + static_cast<float>(quantize_one(p.value(i), s, inv));
+        for (int i = 0; i < 8; ++i) m[i] = static_cast<uint32_t>(quantize_one(p.value(i), s, inv));
     }
     uint2 o;
-    o.x = __byte_perm(__byte_perm(__float_as_uint(m[0]), __float_as_uint(m[1]), 0x0040),
-                      __byte_perm(__float_as_uint(m[2]), __float_as_uint(m[3]), 0x0040), 0x5410);
-    o.y = __byte_perm(__byte_perm(__float_as_uint(m[4]), __float_as_uint(m[5]), 0x0040),
-                      __byte_perm(__float_as_uint(m[6]), __float_as_uint(m[7]), 0x0040), 0x5410);
+    o.x = __byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410);
+    o.y = __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410);
     return o;
 }
 
@@ -160,15 +168,16 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
     ptx::wait_for_dependencies();
 
     // head values before the first 16-byte boundary, whole pieces of eight, tail values
-    const long long cols = live ? p.cols : 0;
-    const int head = static_cast<int>(min(static_cast<long long>(((16u - (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x)) & 15u)) & 15u) / sizeof(T)), cols));
-    const long long pieces = (cols - head) / 8;
-    const long long per_warp = (pieces + WARPS * 32 - 1) / (WARPS * 32) * 32;  // (lane l of step j: piece part * per_warp + 32 j + l)
-    const long long first = min(part * per_warp, pieces), last = min(first + per_warp, pieces);
-    const int tail = static_cast<int>(cols - head - pieces * 8);
+    const int cols = live ? static_cast<int>(p.cols) : 0;
+    const int head = min(static_cast<int>(((16u - (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x)) & 15u)) & 15u) / sizeof(T)), cols);
+    const int pieces = (cols - head) / 8;
+    const int per_warp = (pieces + WARPS * 32 - 1) / (WARPS * 32) * 32;  // (lane l of step j: piece part * per_warp + 32 j + l)
+    const int first = min(part * per_warp, pieces), last = min(first + per_warp, pieces), count = last - first;
+    const int tail = cols - head - pieces * 8;
     // the odd values are the first warp's: lanes 0-7 the head, 8-15 the tail
     const bool odd = part == 0 && ((lane < 8 && lane < head) || (lane >= 8 && lane - 8 < tail));
-    const long long odd_at = lane < 8 ? lane : head + pieces * 8 + (lane - 8);
+    const int odd_at = lane < 8 ? lane : head + pieces * 8 + (lane - 8);
+    const T* from = x + head + (first + lane) * 8ll;
     uint32_t m = 0u;
     float odd_x = 0.0f;
     if (odd) {
@@ -180,15 +189,14 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
     if constexpr (PIECES > 0) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) {
-            const long long i = first + 32 * j + lane;
-            if (i < last) held[j].load(x + head + i * 8);
+            if (32 * j + lane < count) held[j].load(from + 256 * j);
             else held[j].clear();
         }
 #pragma unroll
         for (int j = 0; j < PIECES; ++j) m = max(m, held[j].largest());
     } else {
-        for (long long i = first + lane; i < last; i += 32) {
-            held[0].load(x + head + i * 8);
+        for (int j = 0; j + lane < count; j += 32) {
+            held[0].load(from + 8ll * j);
             m = max(m, held[0].largest());
         }
     }
@@ -206,46 +214,49 @@ __global__ void __launch_bounds__(kQuantizeThreads) quantize_rows_kernel(const Q
     const float inv = __fdiv_rn(1.0f, s);
     if (part == 0 && lane == 0) p.scales[row] = s;
     if (odd) q[odd_at] = finite ? static_cast<signed char>(quantize_one(odd_x, s, inv)) : static_cast<signed char>(0);
+    if (count <= 0) return;
 
     // Piece i makes bytes q[head + 8 i ..]. `shift` of them belong to the aligned eight bytes before the boundary inside
-    // the piece (shift = 0: the piece is aligned as it is).
-    const uint32_t lead = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q + head)) & 7u;
-    const int shift = static_cast<int>((8u - lead) & 7u);
-    uint2 before = make_uint2(0u, 0u);  // the last piece of the step before
-    auto put = [&](long long i0, const QuantizePiece<T>& piece) {
-        const long long i = i0 + lane;
-        const bool valid = i < last;
-        uint2 v = finite ? quantize_piece(piece, s, inv) : make_uint2(0u, 0u);
-        signed char* at = q + head + i * 8;
+    // the piece (shift = 0: the piece is aligned as it is), the rest to those behind it, with `shift` bytes of the next piece.
+    signed char* to = q + head + (first + lane) * 8ll;
+    const int shift = static_cast<int>((8u - (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(to)) & 7u)) & 7u);
+    const bool word = (shift & 4) != 0;
+    const uint32_t bits = 8u * (shift & 3);
+    uint2 carry = make_uint2(0u, 0u);  // lane 0: the last piece of the step before
+    auto put = [&](int j, const QuantizePiece<T>& piece) {  // step of pieces j + lane
+        const bool valid = j + lane < count;
+        const uint2 v = finite ? quantize_piece(piece, s, inv) : make_uint2(0u, 0u);
+        signed char* at = to + 8ll * j;
         if (shift == 0) {
             if (valid) *reinterpret_cast<uint2*>(at) = v;
             return;
         }
         uint2 u;  // the piece before this one
-        u.x = __shfl_up_sync(0xffffffffu, v.x, 1);
-        u.y = __shfl_up_sync(0xffffffffu, v.y, 1);
-        if (lane == 0) u = before;
-        before.x = __shfl_sync(0xffffffffu, v.x, 31);
-        before.y = __shfl_sync(0xffffffffu, v.y, 31);
+        u.x = __shfl_sync(0xffffffffu, v.x, (lane + 31) & 31);
+        u.y = __shfl_sync(0xffffffffu, v.y, (lane + 31) & 31);
+        if (lane == 0) {
+            const uint2 now = u;
+            u = carry;
+            carry = now;
+        }
         if (!valid) return;
         // the aligned eight bytes that end `shift` bytes into this piece
-        if (i == first) {
+        if (j + lane == 0) {
             quantize_store_bytes(at, v, 0, shift);
         } else {
-            const unsigned long long lo = (static_cast<unsigned long long>(u.y) << 32) | u.x, hi = (static_cast<unsigned long long>(v.y) << 32) | v.x;
-            const unsigned long long w = (lo >> (8 * shift)) | (hi << (64 - 8 * shift));
-            *reinterpret_cast<unsigned long long*>(at + shift - 8) = w;
+            const uint32_t w0 = word ? u.y : u.x, w1 = word ? v.x : u.y, w2 = word ? v.y : v.x;
+            *reinterpret_cast<uint2*>(at + shift - 8) = make_uint2(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits));
         }
-        if (i == last - 1) quantize_store_bytes(at, v, shift, 8);
+        if (j + lane == count - 1) quantize_store_bytes(at, v, shift, 8);
     };
     if constexpr (PIECES > 0) {
 #pragma unroll
         for (int j = 0; j < PIECES; ++j)
-            if (first + 32 * j < last) put(first + 32 * j, held[j]);
+            if (32 * j < count) put(32 * j, held[j]);
     } else {
-        for (long long i0 = first; i0 < last; i0 += 32) {
-            if (i0 + lane < last) held[0].load(x + head + (i0 + lane) * 8);
-            put(i0, held[0]);
+        for (int j = 0; j < count; j += 32) {
+            if (j + lane < count) held[0].load(from + 8ll * j);
+            put(j, held[0]);
         }
     }
 }
