@@ -448,19 +448,21 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     const float* first_part = p.parts + plan_slot(first, per) * slot_floats;
     for (int id = threadIdx.x; id < rows * chunks; id += blockDim.x) {
         const int r = id / chunks, ch = id - r * chunks;
-        float mm = first_part[16 * p.size + 2 * r];
-        for (int c = c0 + 1; c <= c1; ++c) mm = fmaxf(mm, p.parts[2ll * c * slot_floats + 16 * p.size + 2 * r]);
-        float ll = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        // a running maximum, so that a part's statistics and values are asked for together
+        float mm = -INFINITY, ll = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int c = c0; c <= c1; ++c) {
             const float* part = c == c0 ? first_part : p.parts + 2ll * c * slot_floats;
-            const float f = mm == -INFINITY ? 0.0f : ptx::exp2_approx(part[16 * p.size + 2 * r] - mm);
             const float4 x = *reinterpret_cast<const float4*>(part + r * p.size + ch * 4);
-            ll += f * part[16 * p.size + 2 * r + 1];
-            acc[0] += f * x.x;
-            acc[1] += f * x.y;
-            acc[2] += f * x.z;
-            acc[3] += f * x.w;
+            const float2 st = *reinterpret_cast<const float2*>(part + 16 * p.size + 2 * r);
+            const float m_new = fmaxf(mm, st.x), base = m_new == -INFINITY ? 0.0f : m_new;
+            const float f = ptx::exp2_approx(mm - base), g = ptx::exp2_approx(st.x - base);
+            mm = m_new;
+            ll = ll * f + st.y * g;
+            acc[0] = acc[0] * f + x.x * g;
+            acc[1] = acc[1] * f + x.y * g;
+            acc[2] = acc[2] * f + x.z * g;
+            acc[3] = acc[3] * f + x.w * g;
         }
         const float inv = ll > 0.0f ? 1.0f / ll : (ll == 0.0f ? 0.0f : ll);
         const int row = row0 + r, tok = row / p.group, h = hk * p.group + row - tok * p.group;
