@@ -338,12 +338,16 @@ def _head_strides(shape, strides):
     return [s if n > 1 else 8 for n, s in zip(shape[:-1], strides)]
 
 
-def _same(tensors, dtype, device, dims):
+def _typed(tensors, dtype, dims):
     for t in tensors:
         if t.dtype != dtype:
             raise BLASError(StatusCode.kInvalidValue)
         if t.dim() != dims or 0 in t.shape:
             raise BLASError(StatusCode.kInvalidDimension)
+
+
+def _placed(tensors, device):
+    for t in tensors:
         if t.device != device or device.type != "cuda":
             raise BLASError(StatusCode.kInvalidMatrixA)
 
@@ -385,7 +389,7 @@ def _attention_call(fn, args, need, device, queue, event):
 
 
 def _attention_plan(Q, K, V, Y, scale, key_mask):
-    _same((Q, K, V, Y), Y.dtype, Y.device, 4)
+    _typed((Q, K, V, Y), Y.dtype, 4)
     b, lq, h, d = Q.shape
     lk, hk = K.shape[1:3]
     if K.shape[0] != b or K.shape[3] != d or V.shape != K.shape or Y.shape != Q.shape or h % hk:
@@ -394,11 +398,10 @@ def _attention_plan(Q, K, V, Y, scale, key_mask):
     if key_mask is not None:
         if key_mask.dtype not in _MASK_TYPES or tuple(key_mask.shape) != (b, lk) or (lk > 1 and key_mask.stride(1) != 1):
             raise BLASError(StatusCode.kInvalidValue)
-        if key_mask.device != Y.device:
-            raise BLASError(StatusCode.kInvalidMatrixA)
         mask_ld = key_mask.stride(0) if b > 1 else lk
     strides = [s for t in (Q, K, V, Y) for s in _head_strides(t.shape, t.stride())]
     args = _ATTENTION_ARGS.pack(int(precision_of(Y)), _default_scale(scale, d), b, lq, lk, h, hk, d, *strides, mask_ld)
+    _placed((Q, K, V, Y) + (() if key_mask is None else (key_mask,)), Y.device)
     return args, lib().dlf_b200_attention_workspace_bytes(b, lq, lk, h, hk, d), b, Y.device
 
 
@@ -430,15 +433,13 @@ def _table_plan(K_pages, V_pages, page_table):
     n, width = page_table.shape
     if page_table.dtype != torch.int32 or (width > 1 and page_table.stride(1) != 1):
         raise BLASError(StatusCode.kInvalidValue)
-    if page_table.device != K_pages.device:
-        raise BLASError(StatusCode.kInvalidMatrixA)
     strides = [_head_strides(t.shape, t.stride()) for t in (K_pages, V_pages)]
     return strides, width, page_table.stride(0) if n > 1 else width
 
 
 def _paged_plan(Q, K_pages, V_pages, page_table, Y, scale):
-    _same((Q, Y), Y.dtype, Y.device, 3)
-    _same((K_pages, V_pages), Y.dtype, Y.device, 4)
+    _typed((Q, Y), Y.dtype, 3)
+    _typed((K_pages, V_pages), Y.dtype, 4)
     b, h, d = Q.shape
     pages, page_size, hk, dk = K_pages.shape
     (ks, vs), width, ld = _table_plan(K_pages, V_pages, page_table)
@@ -446,6 +447,7 @@ def _paged_plan(Q, K_pages, V_pages, page_table, Y, scale):
         raise BLASError(StatusCode.kInvalidDimension)
     args = _PAGED_ARGS.pack(int(precision_of(Y)), _default_scale(scale, d), b, h, hk, d, pages, page_size, width, ld,
                             *_head_strides(Q.shape, Q.stride()), *ks, *vs, *_head_strides(Y.shape, Y.stride()))
+    _placed((Q, K_pages, V_pages, page_table, Y), Y.device)
     return args, lib().dlf_b200_paged_attention_workspace_bytes(b, h, hk, d), b, Y.device
 
 
@@ -467,14 +469,15 @@ def paged_attention(Q, K_pages, V_pages, page_table, lengths, Y, scale=None, que
 
 
 def _append_plan(K, V, K_pages, V_pages, page_table):
-    _same((K, V), K_pages.dtype, K_pages.device, 3)
-    _same((K_pages, V_pages), K_pages.dtype, K_pages.device, 4)
+    _typed((K, V), K_pages.dtype, 3)
+    _typed((K_pages, V_pages), K_pages.dtype, 4)
     pages, page_size, hk, d = K_pages.shape
     (ks, vs), width, ld = _table_plan(K_pages, V_pages, page_table)
     if K.shape != V.shape or tuple(K.shape[1:]) != (hk, d):
         raise BLASError(StatusCode.kInvalidDimension)
     args = _APPEND_ARGS.pack(int(precision_of(K_pages)), K.shape[0], hk, d, page_table.shape[0], pages, page_size, width, ld,
                              *_head_strides(K.shape, K.stride()), *_head_strides(V.shape, V.stride()), *ks, *vs)
+    _placed((K, V, K_pages, V_pages, page_table), K_pages.device)
     return args, K.shape[0], K_pages.device
 
 

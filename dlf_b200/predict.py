@@ -6,7 +6,8 @@ preallocated device tensors and ``predict()`` evaluates the list in order (predi
 The operators are the ones whose work is a contraction or a pooling pass of this library -
 ``Conv`` (predict.h:1258-1286), ``Gemm`` (:1203-1226), ``MatMul`` (:1228-1241), ``MaxPool`` /
 ``AveragePool`` / ``GlobalAveragePool`` / ``GlobalMaxPool`` (:1288-1370) - plus the shape-only
-``Flatten`` / ``Reshape`` / ``Identity``, and the nodes the optimizer folds into a convolution:
+``Flatten`` / ``Reshape`` / ``Identity``, attention over another sequence (``Attention``, in ONNX's form; no counterpart in the
+reference), and the nodes the optimizer folds into a convolution:
 ``BatchNormalization`` and a bias ``Add`` (dlf/src/model/passes.hpp:162-263, 330-403), the ``Add``
 of a residual connection and the ``Relu`` that follows a convolution (one fused launch instead of
 the reference's separate element-wise passes). A node that is none of these is refused when the
@@ -215,6 +216,37 @@ def _broadcast_dims(a, b):
     return tuple(reversed(out))
 
 
+class _AttentionShape:
+    """Sizes of an ``Attention`` node (ONNX: Q, K, V as (batch, heads, length, size) or, with q_num_heads and kv_num_heads, (batch,
+    length, heads * size))."""
+
+    def __init__(self, batch, queries, keys, heads, kv_heads, size, output):
+        self.batch, self.queries, self.keys, self.heads, self.kv_heads, self.size = batch, queries, keys, heads, kv_heads, size
+        self.output = output
+
+
+def _attention_shape(node):
+    q, k, v = (_need(node, i, w) for i, w in enumerate("QKV"))
+    if int(node.get("is_causal", 0)) or float(node.get("softcap", 0.0)) or any(node.input(i) is not None for i in (3, 4, 5)):
+        raise ShapeInferenceError("Attention: masks, past states and softcap are not supported")
+    n = len(q.dims)
+    if n not in (3, 4) or len(k.dims) != n or v.dims != k.dims:
+        raise ShapeInferenceError("Attention: incompatible shapes")
+    if n == 4:
+        (b, h, lq, d), (bk, hk, lk, dk) = q.dims, k.dims
+    else:
+        h, hk = int(node.get("q_num_heads", 0)), int(node.get("kv_num_heads", 0))
+        if h < 1 or hk < 1 or q.dims[2] % h or k.dims[2] % hk:
+            raise ShapeInferenceError("Attention: q_num_heads and kv_num_heads must divide the last dimension")
+        (b, lq), (bk, lk), d, dk = q.dims[:2], k.dims[:2], q.dims[2] // h, k.dims[2] // hk
+    if bk != b or dk != d or h % hk:
+        raise ShapeInferenceError("Attention: incompatible shapes")
+    n_valid = node.input(6)
+    if n_valid is not None and tuple(n_valid.dims or ()) != (b,):
+        raise ShapeInferenceError("Attention: one nonpad_kv_seqlen for each entry of the batch")
+    return _AttentionShape(b, lq, lk, h, hk, d, q.dims)
+
+
 def infer_shapes(graph):
     """Fills in the dims and dtype of every node output (the reference runs
     ShapeInference::infer before it builds the operators, predict.h:2051)."""
@@ -262,6 +294,8 @@ def infer_shapes(graph):
                 dims = dims[:-2] + dims[-1:]
             if len(b_d) == 1:
                 dims = dims[:-1]
+        elif k == "Attention":
+            dims = _attention_shape(node).output
         elif k == "Flatten":
             axis = int(node.get("axis", 1))
             if axis < 0:
@@ -426,7 +460,39 @@ def optimize(graph):
     return graph
 
 
-_OPERATOR_KINDS = ("Conv", "Gemm", "MatMul", "MaxPool", "AveragePool", "GlobalAveragePool", "GlobalMaxPool",
+def int8_product(node):
+    """Whether a product can run in 8-bit integers: rows of activations times a matrix of weights known when the list is built, plus
+    nothing or a bias of the columns."""
+    if node.kind not in ("Gemm", "MatMul") or node.input(0).has_initializer():
+        return False
+    a, w, c = node.input(0), node.input(1), node.input(2)
+    if not w.has_initializer() or len(w.dims) != 2 or len(a.dims) < 2 or 0 in a.dims or 0 in w.dims:
+        return False
+    if node.kind == "MatMul":
+        return True
+    if node.get("transA", 0) or float(node.get("alpha", 1.0)) != 1.0:
+        return False
+    n = node.output(0).dims[-1]
+    return c is None or (c.has_initializer() and float(node.get("beta", 1.0)) == 1.0 and tuple(c.dims) in ((n,), (1, n)))
+
+
+def fuse_relu_into_int8_products(graph):
+    """A Relu that is all that reads such a product becomes a mark on it (its epilogue clamps)."""
+    changed = False
+    for node in list(graph.nodes):
+        if node.kind != "Relu":
+            continue
+        x = node.input(0)
+        if x.node is None or graph.uses(x) != 1 or x.node.attrs.get("relu") or not int8_product(x.node):
+            continue
+        x.node.attrs["relu"] = True
+        graph.replace_all_uses(node.output(0), x)
+        graph.erase(node)
+        changed = True
+    return changed
+
+
+_OPERATOR_KINDS = ("Conv", "Gemm", "MatMul", "Attention", "MaxPool", "AveragePool", "GlobalAveragePool", "GlobalMaxPool",
                    "Flatten", "Reshape")
 
 
@@ -500,6 +566,36 @@ class MatMulOp(Operator):
         m = self.A.shape[-2] if self.A.dim() > 1 else 1
         n = self.B.shape[-1] if self.B.dim() > 1 else 1
         return int(lib().dlf_b200_gemm_workspace_bytes(int(gblas.precision_of(self.C)), m, n, self.A.shape[-1]))
+
+
+class Int8ProductOp(Operator):
+    """A product with known weights in 8-bit integers: the weights rounded once, with a scale for each output channel, the
+    activations row by row when it runs (``tensor.quantize``, ``tensor.matmul_int8``). Two launches, no scratch."""
+
+    def __init__(self, A, W, bias, Y, relu):
+        self.A, self.Y, self.bias, self.relu = A, Y, bias, relu
+        self.W, self.w_scales = linalg.quantize(W)  # (n, k)
+        k = A.shape[-1]
+        self.Q = torch.empty(A.shape[:-1] + ((k + 15) // 16 * 16,), dtype=torch.int8, device=A.device)[..., :k]
+        self.a_scales = torch.empty(A.shape[:-1], dtype=torch.float32, device=A.device)
+
+    def evaluate(self):
+        linalg.quantize(self.A, self.Q, self.a_scales)
+        linalg.matmul_int8(self.Q, self.a_scales, self.W, self.w_scales, self.Y, bias=self.bias, activation="relu" if self.relu else None)
+
+
+class AttentionOp(Operator):
+    """gdnn.attention between (batch, length, heads, size) views of the node's tensors."""
+
+    def __init__(self, Q, K, V, Y, lengths, scale):
+        self.Q, self.K, self.V, self.Y, self.lengths, self.scale = Q, K, V, Y, lengths, scale
+
+    def evaluate(self):
+        gdnn.attention(self.Q, self.K, self.V, self.Y, scale=self.scale, key_lengths=self.lengths)
+
+    def scratch_bytes(self):
+        b, lq, h, d = self.Q.shape
+        return int(lib().dlf_b200_attention_workspace_bytes(b, lq, self.K.shape[1], h, self.K.shape[2], d))
 
 
 class MaxPoolOp(Operator):
@@ -593,14 +689,21 @@ class Predictor:
     unit fetches filter windows from - and runs those operators through the channels-last entries:
     no transposing copy in front of a convolution, TMA-fed operands and TMA stores whatever the
     plane size. Graph inputs and outputs stay NCHW; a copy is inserted where an NCHW value enters the
-    channels-last part."""
+    channels-last part.
 
-    def __init__(self, graph, dtype=torch.float32, device=None, cuda_graph=True, channels_last=True):
+    ``int8`` runs the products with known weights (``Gemm`` / ``MatMul``, with the ``Relu`` that follows one) in 8-bit integers: a
+    scale for each output channel of the weights and, found anew at every ``predict()``, for each row of the activations. The
+    results are those of weights and activations rounded to within half a 127th of their row's largest."""
+
+    def __init__(self, graph, dtype=torch.float32, device=None, cuda_graph=True, channels_last=True, int8=False):
         if dtype not in _TORCH_TYPES:
             raise TypeError("Predictor: T must be float32, float16 or bfloat16")
         self.dtype = dtype
         infer_shapes(graph)
         optimize(graph)
+        self._int8 = bool(int8)
+        if self._int8:
+            fuse_relu_into_int8_products(graph)
         left = unsupported_nodes(graph)
         if left:
             raise NotImplementedError(
@@ -707,7 +810,11 @@ class Predictor:
         if t is None:
             if value.dims is None:
                 raise ShapeInferenceError("value %s has no shape" % value.name)
-            if value.has_initializer():
+            if value.dtype == DataType.INT64:  # (lengths)
+                t = torch.zeros(value.dims, dtype=torch.int32, device=self.device)
+                if value.has_initializer():
+                    t.copy_(torch.from_numpy(np.ascontiguousarray(value.initializer)))
+            elif value.has_initializer():
                 t = torch.from_numpy(np.ascontiguousarray(np.asarray(value.initializer, dtype=np.float64 if
                                      value.dtype == DataType.DOUBLE else np.float32))).to(self.dtype).to(self.device)
             elif like is not None:
@@ -747,6 +854,24 @@ class Predictor:
             res = self._alloc(n.get("residual")) if n.get("residual") is not None else None
             Y = self._alloc(n.output(0))
             return ConvOp(X, W, B, Y, _conv_filter(n, n.input(0).dims, n.input(1).dims), res, bool(n.get("relu")))
+        if self._int8 and int8_product(n):
+            W = self._alloc(n.input(1))
+            if n.kind == "MatMul" or not n.get("transB", 0):
+                W = W.t().contiguous()
+            bias = self._alloc(n.input(2))
+            return Int8ProductOp(self._alloc(n.input(0)), W, None if bias is None else bias.view(-1), self._alloc(n.output(0)), bool(n.get("relu")))
+        if k == "Attention":
+            s = _attention_shape(n)
+            Q, K, V, Y = (self._alloc(v) for v in n.inputs[:3] + [n.output(0)])
+            if len(s.output) == 4:
+                Q, K, V, Y = (x.transpose(1, 2) for x in (Q, K, V, Y))
+            else:
+                Q, Y = (x.view(s.batch, s.queries, s.heads, s.size) for x in (Q, Y))
+                K, V = (x.view(s.batch, s.keys, s.kv_heads, s.size) for x in (K, V))
+            if self.dtype == torch.float32 or s.size > 128 or s.size % 8:
+                raise NotImplementedError("Attention: float16 or bfloat16 and heads of a multiple of 8 values up to 128")
+            scale = float(n.get("scale", 0.0)) or None
+            return AttentionOp(Q, K, V, Y, self._alloc(n.input(6)), scale)
         if k == "Gemm":
             A, B, C = self._alloc(n.input(0)), self._alloc(n.input(1)), self._alloc(n.input(2))
             return GemmOp(A, B, C, self._alloc(n.output(0)), n.get("alpha", 1.0), n.get("beta", 1.0),
@@ -773,7 +898,7 @@ class Predictor:
         src = data if isinstance(data, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(data))
         if tuple(src.shape) != tuple(dst.shape):
             raise ShapeInferenceError("input %d: shape %r expected, %r given" % (i, tuple(dst.shape), tuple(src.shape)))
-        dst.copy_(src.to(self.dtype), non_blocking=True)
+        dst.copy_(src.to(dst.dtype), non_blocking=True)
 
     def input(self, i):
         """The device tensor behind graph input i, for callers that fill it on the device."""

@@ -272,12 +272,11 @@ def _rows(t, what):
     return m, n, ld if m > 1 else max(ld, n)
 
 
-def _typed(what, device, *tensors):
-    for t, dtype in tensors:
-        if t.dtype != dtype:
-            raise _gblas.BLASError(_gblas.StatusCode.kInvalidValue)
-        if t.device != device or device.type != "cuda":
-            raise _gblas.BLASError(_gblas.StatusCode.kInvalidMatrixA)
+def _typed(device, *tensors):
+    if any(t.dtype != dtype for t, dtype in tensors):
+        raise _gblas.BLASError(_gblas.StatusCode.kInvalidValue)
+    if device.type != "cuda" or any(t.device != device for t, _ in tensors):
+        raise _gblas.BLASError(_gblas.StatusCode.kInvalidMatrixA)
 
 
 def _quantize_plan(X, Q, scales):
@@ -286,9 +285,10 @@ def _quantize_plan(X, Q, scales):
     if scales.shape != X.shape[:-1] or not scales.is_contiguous():
         raise ShapeError("quantize: one scale for each row of X, contiguous")
     prec = _gblas.precision_of(X)
-    _typed("quantize", X.device, (X, X.dtype), (Q, torch.int8), (scales, torch.float32))
     m, n, x_ld = _rows(X, "quantize")
-    return int(prec), m, n, x_ld, _rows(Q, "quantize")[2], X.device
+    q_ld = _rows(Q, "quantize")[2]
+    _typed(X.device, (X, X.dtype), (Q, torch.int8), (scales, torch.float32))
+    return int(prec), m, n, x_ld, q_ld, X.device
 
 
 def quantize(X, Q=None, scales=None, queue=None, event=None):
@@ -326,11 +326,12 @@ def _int8_plan(A, a_scales, B, b_scales, C, bias, activation):
     if activation not in (None, "relu"):
         raise _gblas.BLASError(_gblas.StatusCode.kInvalidValue)
     prec = _gblas.precision_of(C)
-    _typed("matmul_int8", C.device, (C, C.dtype), (A, torch.int8), (B, torch.int8), (a_scales, torch.float32), (b_scales, torch.float32),
-           *([(bias, C.dtype)] if bias is not None else []))
     m, k, a_ld = _rows(A, "matmul_int8")
     n, _, b_ld = _rows(B, "matmul_int8")
-    return int(prec), m, n, k, a_ld, b_ld, 1 if activation == "relu" else 0, _rows(C, "matmul_int8")[2], C.device
+    c_ld = _rows(C, "matmul_int8")[2]
+    _typed(C.device, (C, C.dtype), (A, torch.int8), (B, torch.int8), (a_scales, torch.float32), (b_scales, torch.float32),
+           *([(bias, C.dtype)] if bias is not None else []))
+    return int(prec), m, n, k, a_ld, b_ld, 1 if activation == "relu" else 0, c_ld, C.device
 
 
 def matmul_int8(A, a_scales, B, b_scales, C=None, bias=None, activation=None, dtype=torch.float32, queue=None, event=None):
