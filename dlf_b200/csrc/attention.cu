@@ -125,8 +125,11 @@ int tiles_launch(const TilesParams& p, const CUtensorMap& q, const CUtensorMap& 
     return kSuccess;
 }
 
-// few query rows for each kv head: the kernel that reads the keys once for 16 rows
-bool few_rows(size_t queries, size_t group) { return queries * group <= 16; }
+// Few queries: the kernel that runs through the keys for 16 rows (a token's heads of a group are rows too). It does as much work as
+// there are rows, the other one as if every head had 128 queries at least; with 32 entries of 1500 keys and 8 heads (us, this
+// kernel and the other): heads of 64 24 and 47 (16 queries), 33 and 47 (32), 53 and 48 (64); heads of 128 45 and 59 (16), 73 and
+// 60 (32). 32 query heads on one kv head, 1 query: 13 and 128.
+bool few_rows(size_t queries, size_t size) { return queries <= (size <= 64 ? 32 : 16); }
 
 int head_args(int dtype, size_t heads, size_t kv_heads, size_t size) {
     if (dtype != DLF_B200_HALF && dtype != DLF_B200_BFLOAT16) return kNotImplemented;
@@ -142,7 +145,7 @@ extern "C" {
 size_t dlf_b200_attention_workspace_bytes(size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size) {
     (void)batch;
     if (kv_heads == 0 || heads % kv_heads != 0) return 0;
-    return few_rows(queries, heads / kv_heads) ? decode_workspace(size) : tiles_workspace(keys, size);
+    return few_rows(queries, size) ? decode_workspace(size) : tiles_workspace(keys, size);
 }
 
 int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -156,7 +159,7 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     if (q == nullptr) return kInvalidMatrixA;
     if (k == nullptr || v == nullptr) return kInvalidMatrixB;
     if (y == nullptr) return kInvalidMatrixC;
-    if (key_mask != nullptr && key_mask_ld < keys && batch > 1) return kInvalidLeadDimB;
+    if (key_mask != nullptr && key_mask_ld < keys && key_mask_ld != 0 && batch > 1) return kInvalidLeadDimB;
     if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(y) ||
         !strides_ok({q_strides[0], q_strides[1], q_strides[2], k_strides[0], k_strides[1], k_strides[2], v_strides[0], v_strides[1], v_strides[2],
                      y_strides[0], y_strides[1], y_strides[2]}))
@@ -166,11 +169,11 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     if ((keys > 1 && (k_strides[1] == 0 || v_strides[1] == 0)) || (kv_heads > 1 && (k_strides[2] == 0 || v_strides[2] == 0))) return kInvalidLeadDimB;
     const bool bf16 = dtype == DLF_B200_BFLOAT16;
     const size_t group = heads / kv_heads;
-    const bool few = few_rows(queries, group);
+    const bool few = few_rows(queries, size);
     const size_t need = dlf_b200_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, size);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return kInsufficientMemoryTemp;
     const long long items = static_cast<long long>((queries + 255) / 256) * static_cast<long long>(heads) * static_cast<long long>(batch);
-    if (static_cast<double>(items) * (static_cast<double>(keys) / kTileKeys + 1.0) > 2147483647.0 || static_cast<double>(batch) * heads * (keys / kDecodeUnit + 1.0) > 2147483647.0) return kInvalidDimension;
+    if (static_cast<double>(items) * (static_cast<double>(keys) / kTileKeys + 1.0) > 2147483647.0 || 2.0 * static_cast<double>(batch) * heads * (keys / kDecodeUnit + 1.0) > 2147483647.0) return kInvalidDimension;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     StreamDevice guard(s);
     if (guard.rc != kSuccess) return guard.rc;
@@ -326,6 +329,8 @@ int dlf_b200_paged_append(const dlf_b200_paged_append_args* args, void* stream) 
         !strides_ok({k_strides[0], k_strides[1], v_strides[0], v_strides[1], kp_strides[0], kp_strides[1], kp_strides[2], vp_strides[0], vp_strides[1],
                      vp_strides[2]}))
         return kNotImplemented;
+    for (const size_t* st : {&kp_strides[0], &vp_strides[0]})  // (a place of its own for every token and head)
+        if ((num_pages > 1 && st[0] == 0) || (page_size > 1 && st[1] == 0) || (kv_heads > 1 && st[2] == 0)) return kInvalidLeadDimC;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     StreamDevice guard(s);
     if (guard.rc != kSuccess) return guard.rc;

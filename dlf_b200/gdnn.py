@@ -412,7 +412,8 @@ def attention(Q, K, V, Y, scale=None, key_lengths=None, key_mask=None, queue=Non
 
     ``key_lengths`` (batch, int32) and ``key_mask`` (batch, keys; bool or uint8, 0 = left out) say which keys count; those that do not
     may hold anything. A query with no key gets zeros. Any strides that are multiples of 8 elements, over 16-byte aligned
-    addresses, with a head's values contiguous; Q, K and V may be shared by the batch (expanded)."""
+    addresses, with a head's values contiguous; Q, K, V and the mask may be shared by the batch (expanded). Y must not overlap the
+    inputs."""
     key = (Q.dtype, K.dtype, V.dtype, Y.dtype, Q.device, K.device, V.device, Y.device, Q.shape, K.shape, V.shape, Y.shape, Q.stride(), K.stride(),
            V.stride(), Y.stride(), scale,
            None if key_mask is None else (key_mask.dtype, key_mask.device, key_mask.shape, key_mask.stride()))

@@ -280,8 +280,8 @@ size_t dlf_b200_gemm_int8_workspace_bytes(size_t m, size_t n, size_t k, const si
  *
  * dlf_b200_attention: Q and Y are (batch, queries, heads, size) with strides {batch, token, head}, K and V (batch, keys,
  * kv_heads, size) with theirs; a batch stride of 0 shares Q, K or V between the batch's entries. `key_lengths` (batch, device, or
- * NULL): keys of each entry that count, the rest is padding. `key_mask` (batch, keys, bytes; lines key_mask_ld apart; device, or
- * NULL): 0 = the key does not count. `workspace`: dlf_b200_attention_workspace_bytes bytes of device memory (0 where none is
+ * NULL): keys of each entry that count, the rest is padding. `key_mask` (batch, keys, bytes; lines key_mask_ld apart, 0 = one line for
+ * all; device, or NULL): 0 = the key does not count. `workspace`: dlf_b200_attention_workspace_bytes bytes of device memory (0 where none is
  * needed). Y must not overlap the inputs.
  *
  * dlf_b200_paged_attention: one query token for each sequence. Q and Y are (batch, heads, size) with strides {batch, head}; the
@@ -338,7 +338,8 @@ const char* dlf_b200_status_string(int status);
 
 /* Synchronises the current device and reads-and-clears its kernel status word: 0 when every
  * kernel since the last call ran to completion, non-zero when a bounded device-side wait gave
- * up (bit 0). Kernels never trap or spin forever; this is how such a failure is reported. */
+ * up (bit 0). Kernels never trap or spin forever; this is how such a failure is reported. Bit 1: attention met a length, a
+ * position or a page that does not exist (and left it out). */
 int dlf_b200_device_status(int* device_status);
 
 /* Tuning overrides for experiments, for every following call of this process: force the N-tile

@@ -182,7 +182,7 @@ def test_product_wait_that_runs_out_is_reported():
     """One tile whose last hand-over is left out (a test aid): the kernel gives up, returns and reports; the next call is sound."""
     a, b = torch.ones(8, 64, dtype=torch.int8).cuda(), torch.ones(8, 64, dtype=torch.int8).cuda()
     s = torch.ones(8).cuda()
-    q = torch.zeros(1, 30, 1, 64, dtype=torch.float16, device="cuda")
+    q = torch.zeros(1, 40, 1, 64, dtype=torch.float16, device="cuda")
     tensor.matmul_int8(a, s, b, s)
     gdnn.attention(q, q, q, torch.empty_like(q))
     assert dlf_b200.device_status() == 0
@@ -236,7 +236,7 @@ def _check_attention(b, lq, lk, h, hk, d, dtype, padding="none", garbage=True, s
 
     kb = 1 if shared else b
     if layout == "packed":  # keys and values of one projection
-        q, (k, v) = rand(b, lq, h, d), rand(kb, lk, 2, hk, d).unbind(2)
+        q, (k, v) = rand(1 if shared else b, lq, h, d).expand(b, -1, -1, -1), rand(kb, lk, 2, hk, d).unbind(2)
         y = torch.full((b, lq, h, d), 7.0, dtype=dtype, device="cuda")
     else:  # heads before tokens, lines with room behind them
         q, k, v = (rand(x, n, m, d + 8)[..., :d].transpose(1, 2) for x, n, m in ((b, h, lq), (kb, hk, lk), (kb, hk, lk)))
@@ -249,6 +249,9 @@ def _check_attention(b, lq, lk, h, hk, d, dtype, padding="none", garbage=True, s
         if b > 1:
             lengths[b - 1] = 0
         keep &= torch.arange(lk, device="cuda") < lengths.unsqueeze(1)
+    if padding == "one mask":
+        mask = (torch.rand(1, lk, generator=g, device="cuda") < 0.6).expand(b, -1)
+        keep &= mask
     if padding in ("mask", "both"):
         mask = torch.rand(b, lk, generator=g, device="cuda") < 0.6
         if b > 1:
@@ -258,7 +261,7 @@ def _check_attention(b, lq, lk, h, hk, d, dtype, padding="none", garbage=True, s
         k[~keep], v[~keep] = math.nan, math.inf
     kx, vx = (k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1)) if shared else (k, v)
     gdnn.attention(q, kx, vx, y, scale=scale, key_lengths=lengths, key_mask=mask)
-    few = lq * (h // hk) <= 16
+    few = lq <= (32 if d <= 64 else 16)  # the kernel that keeps P in two parts
     for i in range(b):
         want, a, e = _attention_want(q[i], kx[i], vx[i], keep[i], scale or 1 / math.sqrt(d))
         _check_rows(y[i], want, a, e, dtype, _half_step(dtype) ** 2 if few else _half_step(dtype))
@@ -297,6 +300,7 @@ def test_attention_layouts_and_shared_states(lq, d):
     _check_attention(3, lq, 190, 4, 2, d, torch.bfloat16, "lengths", layout="heads first")
     _check_attention(3, lq, 190, 4, 2, d, torch.bfloat16, "mask", layout="heads first")
     _check_attention(3, lq, 190, 4, 2, d, torch.float16, "lengths", shared=True)
+    _check_attention(3, lq, 190, 4, 2, d, torch.float16, "one mask", shared=True)
     _check_attention(1, lq, 190, 4, 1, d, torch.float16, layout="heads first")
 
 
@@ -313,7 +317,7 @@ def test_attention_scores_that_grow_and_scales(lq, d):
             y = torch.empty_like(q)
             gdnn.attention(q, order, v, y, scale=0.5)
             want, a, e = _attention_want(q[0], order[0], v[0], torch.ones(700, dtype=torch.bool, device="cuda"), 0.5)
-            _check_rows(y[0], want, a, e, dtype, _half_step(dtype) if lq > 16 else _half_step(dtype) ** 2)
+            _check_rows(y[0], want, a, e, dtype, _half_step(dtype) if lq > 32 else _half_step(dtype) ** 2)
 
 
 @pytest.mark.parametrize("b,lq,lk,h,hk,d", [(1, 256, 40000, 1, 1, 64), (1, 40, 9000, 2, 1, 128), (2, 300, 5000, 3, 1, 80), (1, 1, 60000, 4, 1, 128)])
@@ -542,6 +546,9 @@ def test_paged_refusals_on_the_device():
     refused(StatusCode.kInvalidDimension, q[:, :3], kp, vp, table, n, y[:, :3])
     refused(StatusCode.kInvalidMatrixA, q, kp, vp, table.cpu(), n, y)
     refused(StatusCode.kNotImplemented, q.float(), kp.float(), vp.float(), table, n, y.float())
+    with pytest.raises(BLASError) as e:
+        gdnn.paged_append(kp[0, :2], vp[0, :2], kp[:1].expand(4, -1, -1, -1), vp[:4], table, n)
+    assert e.value.status == StatusCode.kInvalidLeadDimC  # pages that are one
     with pytest.raises(BLASError) as e:
         gdnn.paged_append(kp[0], vp[0], kp, vp, table, torch.zeros(10, dtype=torch.int32, device="cuda"))
     assert e.value.status == StatusCode.kInvalidDimension  # more tokens than sequences
@@ -853,7 +860,7 @@ def test_rows_and_pages_beyond_32_bit_offsets():
         gdnn.attention(q, far, far, y)
         for i in range(2):
             want, a, e = _attention_want(q[i], far[i], far[i], torch.ones(200, dtype=torch.bool, device="cuda"), 1 / math.sqrt(d))
-            _check_rows(y[i], want, a, e, torch.float16, _half_step(torch.float16) if lq > 16 else _half_step(torch.float16) ** 2)
+            _check_rows(y[i], want, a, e, torch.float16, _half_step(torch.float16) if lq > 32 else _half_step(torch.float16) ** 2)
     del kp, vp, far, k, v
     rows = torch.zeros(3, (1 << 31) + 64, dtype=torch.int8, device="cuda")  # products whose lines lie that far apart
     a = rows[:, :200]
