@@ -241,9 +241,11 @@ def _attention_shape(node):
         (b, lq), (bk, lk), d, dk = q.dims[:2], k.dims[:2], q.dims[2] // h, k.dims[2] // hk
     if bk != b or dk != d or h % hk:
         raise ShapeInferenceError("Attention: incompatible shapes")
+    if len(node.outputs) > 1:
+        raise ShapeInferenceError("Attention: present states and scores are not supported")
     n_valid = node.input(6)
-    if n_valid is not None and tuple(n_valid.dims or ()) != (b,):
-        raise ShapeInferenceError("Attention: one nonpad_kv_seqlen for each entry of the batch")
+    if n_valid is not None and (n_valid.node is not None or tuple(n_valid.dims or ()) != (b,)):
+        raise ShapeInferenceError("Attention: one nonpad_kv_seqlen for each entry of the batch, an input or known")
     return _AttentionShape(b, lq, lk, h, hk, d, q.dims)
 
 
@@ -460,6 +462,9 @@ def optimize(graph):
     return graph
 
 
+_INT8_DEPTH = 131071  # the deepest product whose 32-bit sums are exact
+
+
 def int8_product(node):
     """Whether a product can run in 8-bit integers: rows of activations times a matrix of weights known when the list is built, plus
     nothing or a bias of the columns."""
@@ -467,6 +472,8 @@ def int8_product(node):
         return False
     a, w, c = node.input(0), node.input(1), node.input(2)
     if not w.has_initializer() or len(w.dims) != 2 or len(a.dims) < 2 or 0 in a.dims or 0 in w.dims:
+        return False
+    if a.dims[-1] > _INT8_DEPTH and not node.get("transA", 0):
         return False
     if node.kind == "MatMul":
         return True
@@ -582,6 +589,11 @@ class Int8ProductOp(Operator):
     def evaluate(self):
         linalg.quantize(self.A, self.Q, self.a_scales)
         linalg.matmul_int8(self.Q, self.a_scales, self.W, self.w_scales, self.Y, bias=self.bias, activation="relu" if self.relu else None)
+
+
+def _as_lengths(t):
+    """Whole numbers as 32-bit ones, cut to their range (below 0 there is only "none")."""
+    return t.to(torch.int64).clamp(-1, 2 ** 31 - 1).to(torch.int32)
 
 
 class AttentionOp(Operator):
@@ -712,6 +724,7 @@ class Predictor:
         self.graph = graph
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self._data = {}
+        self._lengths = {id(n.input(6)) for n in graph.nodes if n.kind == "Attention" and n.input(6) is not None}
         self._nhwc_copy = {}
         self._pre_ops = []
         self._nhwc = self._assign_layouts(graph) if channels_last and dtype != torch.float32 else set()
@@ -810,10 +823,10 @@ class Predictor:
         if t is None:
             if value.dims is None:
                 raise ShapeInferenceError("value %s has no shape" % value.name)
-            if value.dtype == DataType.INT64:  # (lengths)
+            if id(value) in self._lengths:
                 t = torch.zeros(value.dims, dtype=torch.int32, device=self.device)
                 if value.has_initializer():
-                    t.copy_(torch.from_numpy(np.ascontiguousarray(value.initializer)))
+                    t.copy_(_as_lengths(torch.from_numpy(np.ascontiguousarray(value.initializer))))
             elif value.has_initializer():
                 t = torch.from_numpy(np.ascontiguousarray(np.asarray(value.initializer, dtype=np.float64 if
                                      value.dtype == DataType.DOUBLE else np.float32))).to(self.dtype).to(self.device)
@@ -898,7 +911,8 @@ class Predictor:
         src = data if isinstance(data, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(data))
         if tuple(src.shape) != tuple(dst.shape):
             raise ShapeInferenceError("input %d: shape %r expected, %r given" % (i, tuple(dst.shape), tuple(src.shape)))
-        dst.copy_(src.to(dst.dtype), non_blocking=True)
+        src = _as_lengths(src) if dst.dtype == torch.int32 else src.to(self.dtype)
+        dst.copy_(src, non_blocking=True)
 
     def input(self, i):
         """The device tensor behind graph input i, for callers that fill it on the device."""

@@ -519,6 +519,31 @@ def test_paged_append_leaves_out_what_does_not_exist():
     assert torch.equal(kp, before_k) and torch.equal(vp, before_v)
 
 
+def test_a_padded_batch_appends_and_attends_without_a_report():
+    """Sequences of length 0 (positions -1) between others, their table entries anything."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    table, kp, vp = _cache(g, 5, 40, 10, 2, 64, torch.float16)
+    n = torch.tensor([0, 17, 0, 40, -1], dtype=torch.int32, device="cuda")
+    table[n <= 0] = 2 ** 31 - 1
+    q, k = (torch.randn(5, h, 64, generator=g, device="cuda").half() for h in (4, 2))
+    want_k = kp.clone()
+    for i in (1, 3):
+        last = int(n[i]) - 1
+        want_k[table[i, last // 10].long(), last % 10] = k[i]
+    gdnn.paged_append(k, k, kp, vp, table, n - 1)
+    y = torch.full_like(q, float("nan"))
+    gdnn.paged_attention(q, kp, vp, table, n, y)
+    assert dlf_b200.device_status() == 0
+    assert torch.equal(kp, want_k)
+    for i in range(5):
+        if n[i] <= 0:
+            assert bool((y[i] == 0).all())
+        else:
+            flat = kp[table[i].long()].reshape(-1, 2, 64)[:n[i]], vp[table[i].long()].reshape(-1, 2, 64)[:n[i]]
+            want, a, e = _attention_want(q[i:i + 1], *flat, torch.ones(int(n[i]), dtype=torch.bool, device="cuda"), 1 / 8)
+            _check_rows(y[i:i + 1], want, a, e, torch.float16, _half_step(torch.float16) ** 2)
+
+
 def test_paged_append_the_same_place_twice_holds_one_of_the_two_in_every_piece():
     table, kp, vp = _cache(torch.Generator(device="cuda").manual_seed(7), 1, 16, 16, 1, 64, torch.float16)
     k = torch.stack([torch.full((1, 64), 1.0), torch.full((1, 64), 2.0)]).cuda().half()
@@ -825,6 +850,43 @@ def test_predictor_products_in_8_bit_integers(dtype):
             tol = 3 * 2.0 ** -24 * (scaled.abs() + want.abs()) + _half_step(dtype) * want.abs() * (1 + 2.0 ** -20)
             assert bool(((got.double() - want).abs() <= tol).all())
     assert [type(op).__name__ for op in build(False).operators] == ["GemmOp", "GemmOp", "MatMulOp"]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_predictor_8_bit_product_behind_channels_last_convolutions(dtype):
+    """Convolutions whose values stay channels-last, Flatten, Gemm: what the product is given is in the graph's order."""
+    rng = np.random.default_rng(1)
+    wc, wg = rng.standard_normal((16, 8, 3, 3)).astype(np.float32), rng.standard_normal((16 * 36, 24)).astype(np.float32)
+
+    def build(int8):
+        g = predict.Graph()
+        n = g.append("Conv", kernel_shape=(3, 3), pads=(1, 1, 1, 1))
+        n.addInput(g.addInput("x", predict.DataType.FLOAT, (2, 8, 6, 6)))
+        n.addInput(g.addInitializer("wc", wc))
+        h = n.addOutput("h")
+        n = g.append("Flatten")
+        n.addInput(h)
+        f = n.addOutput("f")
+        n = g.append("Gemm")
+        n.addInput(f)
+        n.addInput(g.addInitializer("wg", wg))
+        for v in (f, n.addOutput("y")):
+            g.addOutput(v)
+        return predict.Predictor(g, dtype, int8=int8)
+
+    x = _rand(3, 2, 8, 6, 6).to(dtype)
+    p, plain = build(True), build(False)
+    for _ in range(3):
+        for r in (p, plain):
+            r.set(0, x)
+            r.predict()
+        given, got = (torch.from_numpy(p.get(i)).to(dtype) for i in range(2))
+        assert torch.equal(given, torch.from_numpy(plain.get(0)).to(dtype))
+        qa, sa = _quantized(given)
+        qw, sw = _quantized(torch.from_numpy(wg).t().to(dtype).contiguous())
+        want = (qa.double() @ qw.double().t()) * sa.double().unsqueeze(1) * sw.double()
+        tol = 3 * 2.0 ** -24 * 2 * want.abs() + _half_step(dtype) * want.abs() * (1 + 2.0 ** -20)
+        assert bool(((got.double() - want).abs() <= tol).all())
 
 
 # ---------------------------------------------------------------------------------------------

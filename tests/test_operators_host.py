@@ -266,3 +266,106 @@ def test_which_products_run_in_8_bit_integers():
               graph("MatMul", (8,), (8, 6))):
         assert not predict.int8_product(g.nodes[0])
         assert not predict.fuse_relu_into_int8_products(g) and predict.unsupported_nodes(g)
+
+
+def test_products_deeper_than_exact_sums_stay_in_floating_point():
+    for k, exact in ((131071, True), (131072, False)):
+        g = predict.Graph()
+        n = g.append("MatMul")
+        n.addInput(g.addInput("a", predict.DataType.FLOAT, (2, k)))
+        n.addInput(g.addInitializer("w", np.zeros((k, 1), np.float32)))
+        g.addOutput(n.addOutput("y"))
+        predict.infer_shapes(g)
+        assert predict.int8_product(g.nodes[0]) == exact
+
+
+def test_attention_nodes_refuse_outputs_and_lengths_that_are_not_there():
+    def graph():
+        g = predict.Graph()
+        node = g.append("Attention")
+        for name in "qkv":
+            node.addInput(g.addInput(name, predict.DataType.FLOAT, (2, 4, 5, 64)))
+        node.addOutput("y")
+        return g, node
+
+    g, node = graph()
+    node.addOutput("present_key")
+    with pytest.raises(predict.ShapeInferenceError):
+        predict.infer_shapes(g)
+    g, node = graph()
+    flat = predict.Node("Flatten", {"axis": 0})
+    g.nodes.insert(0, flat)
+    flat.addInput(g.addInput("n", predict.DataType.FLOAT, (2, 1)))
+    for _ in range(3):
+        node.addInput(None)
+    node.addInput(flat.addOutput("lengths"))  # computed in floating point
+    with pytest.raises(predict.ShapeInferenceError):
+        predict.infer_shapes(g)
+
+
+def test_integers_of_a_graph_keep_the_lists_type_unless_they_are_lengths():
+    """Weights and inputs that are whole numbers are operands like others; lengths are 32-bit integers, cut to their range."""
+    g = predict.Graph()
+    n = g.append("MatMul")
+    n.addInput(g.addInput("a", predict.DataType.INT64, (3, 4)))
+    n.addInput(g.addInitializer("w", np.arange(8).reshape(4, 2)))
+    g.addOutput(n.addOutput("p"))
+    node = g.append("Attention")
+    for name in "qkv":
+        node.addInput(g.addInput(name, predict.DataType.FLOAT, (3, 2, 5, 64)))
+    for _ in range(3):
+        node.addInput(None)
+    node.addInput(g.addInitializer("n", np.array([2 ** 32 + 5, -(2 ** 40), 4])))
+    g.addOutput(node.addOutput("y"))
+    p = predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False)
+    ops = {type(op).__name__: op for op in p.operators}
+    assert ops["MatMulOp"].A.dtype == ops["MatMulOp"].B.dtype == torch.float16
+    assert ops["MatMulOp"].B.tolist() == [[0, 1], [2, 3], [4, 5], [6, 7]]
+    assert ops["AttentionOp"].lengths.dtype == torch.int32 and ops["AttentionOp"].lengths.tolist() == [2 ** 31 - 1, -1, 4]
+    p.set(0, torch.arange(12).view(3, 4))
+    assert p.input(0).tolist() == torch.arange(12).view(3, 4).tolist()
+
+
+def test_lengths_that_are_set_are_cut_to_32_bits():
+    g = predict.Graph()
+    node = g.append("Attention")
+    for name in "qkv":
+        node.addInput(g.addInput(name, predict.DataType.FLOAT, (2, 2, 5, 64)))
+    for _ in range(3):
+        node.addInput(None)
+    node.addInput(g.addInput("n", predict.DataType.INT64, (2,)))
+    g.addOutput(node.addOutput("y"))
+    p = predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False)
+    for given, want in ((torch.tensor([2 ** 32 + 3, -(2 ** 33)]), [2 ** 31 - 1, -1]), (torch.tensor([3, -1], dtype=torch.int8), [3, -1])):
+        p.set(3, given)
+        assert p.input(3).tolist() == want
+
+
+def test_attention_scale_beyond_single_precision_is_refused(built_lib):
+    assert _attention(built_lib, scale=3.0e38) == StatusCode.kInvalidValue  # (times log2 e)
+    assert _paged(built_lib, scale=3.0e38) == StatusCode.kInvalidValue
+    for scale in (3.0e38, 1e300):
+        with pytest.raises(BLASError):
+            gdnn._default_scale(scale, 64)
+
+
+def test_a_scale_in_a_tensor_is_read_at_every_call(built_lib, monkeypatch):
+    seen = []
+    for plans in ("_ATTENTION_PLANS", "_PAGED_PLANS"):
+        monkeypatch.setattr(gdnn, plans, gblas._Plans())
+    monkeypatch.setattr(gdnn, "_placed", lambda *a: None)
+    monkeypatch.setattr(gdnn, "_attention_call", lambda fn, args, *rest: seen.append(gdnn._ATTENTION_ARGS.unpack_from(args)[1]))
+    q, scale = torch.zeros(1, 3, 2, 64, dtype=torch.float16), torch.tensor(0.5)
+    for value in (0.5, 0.25):
+        scale.fill_(value)
+        gdnn.attention(q, q, q, torch.empty_like(q), scale=scale)
+        gdnn.paged_attention(q[0], q, q, torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32), torch.empty_like(q[0]), scale=scale)
+    assert seen == [0.5, 0.5, 0.25, 0.25]
+
+
+def test_streams_of_another_device_are_refused():
+    class Queue:
+        device_index, cuda_stream = 1, 0
+
+    _refused(StatusCode.kInvalidValue, gblas._operator_stream, Queue(), torch.device("cuda", 0))
+    assert gblas._operator_stream(Queue(), torch.device("cuda", 1)) == 0
