@@ -16,6 +16,7 @@ using namespace dlfb200;
 
 namespace {
 
+constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kDecodeLeast = 2;    // units a CTA takes at least
 constexpr int kB200Sms = 148;  // for sizes that are asked for without a device at hand
 
@@ -50,6 +51,7 @@ int attention_device(const OperatorDevice& dev) {
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool scale_ok(float scale) { return scale > 0.0f && !std::isinf(scale * kLog2e); }
 // strides that 16-byte pieces and tensor maps take
 bool strides_ok(std::initializer_list<size_t> s) {
     for (size_t x : s)
@@ -155,7 +157,7 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     int rc = head_args(dtype, heads, kv_heads, size);
     if (rc != kSuccess) return rc;
     if (batch == 0 || queries == 0 || keys == 0 || batch > 65535 || queries > INT_MAX / 2 || keys > INT_MAX / 2) return kInvalidDimension;
-    if (!(scale > 0.0f) || std::isinf(scale)) return kInvalidValue;
+    if (!scale_ok(scale)) return kInvalidValue;
     if (q == nullptr) return kInvalidMatrixA;
     if (k == nullptr || v == nullptr) return kInvalidMatrixB;
     if (y == nullptr) return kInvalidMatrixC;
@@ -183,7 +185,7 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     rc = attention_device(dev);
     if (rc != kSuccess) return rc;
     clear_stale_error();
-    const float c = scale * 1.44269504088896340736f;
+    const float c = scale * kLog2e;
     if (few) {
         DecodeParams p{};
         p.q = static_cast<const char*>(q);
@@ -261,7 +263,7 @@ int dlf_b200_paged_attention(const dlf_b200_paged_attention_args* args, void* wo
     if (batch == 0 || num_pages == 0 || page_size == 0 || table_width == 0 || batch > 65535 || num_pages > INT_MAX || page_size > INT_MAX ||
         static_cast<double>(table_width) * static_cast<double>(page_size) > INT_MAX / 2)
         return kInvalidDimension;
-    if (!(scale > 0.0f) || std::isinf(scale)) return kInvalidValue;
+    if (!scale_ok(scale)) return kInvalidValue;
     if (q == nullptr) return kInvalidMatrixA;
     if (k_pages == nullptr || v_pages == nullptr || page_table == nullptr || lengths == nullptr)
         return kInvalidMatrixB;
@@ -305,7 +307,7 @@ int dlf_b200_paged_attention(const dlf_b200_paged_attention_args* args, void* wo
     p.keys = static_cast<int>(table_width * page_size);
     p.ctas = std::min(dev.num_sms, kB200Sms);
     p.least = kDecodeLeast;
-    p.c = scale * 1.44269504088896340736f;
+    p.c = scale * kLog2e;
     p.parts = static_cast<float*>(workspace);
     p.status = dev.status;
     return decode_any(p, dtype == DLF_B200_BFLOAT16, s);

@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
 }
 
 // New keys and values into a paged cache: token i of K and V to position positions[i] of sequence sequences[i] (null: i). Tokens
-// whose sequence, position or page does not exist are left out and reported. A thread moves 16 bytes; HBM-bound where there are
+// whose sequence, position or page does not exist are left out and reported; those with positions below 0 are padding, left out. A thread moves 16 bytes; HBM-bound where there are
 // many tokens, a launch's latency where there are few.
 struct AppendParams {
     const char* k;
@@ -501,7 +501,8 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
         const int h = rest / chunks, ch = rest - h * chunks;
         const int pos = p.positions[tok], seq = p.sequences != nullptr ? p.sequences[tok] : tok;
         const int pg = pos / p.page_size, place = pos - pg * p.page_size;
-        if (pos < 0 || seq < 0 || seq >= p.batch || pg >= p.table_width) {
+        if (pos < 0) continue;  // padding
+        if (seq < 0 || seq >= p.batch || pg >= p.table_width) {
             bad = true;
             continue;
         }

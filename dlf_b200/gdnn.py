@@ -364,7 +364,7 @@ def _device_ints(t, count, device):
 
 def _default_scale(scale, size):
     scale = 1.0 / math.sqrt(size) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
+    if not 0.0 < scale * 1.4426950408889634 <= 3.4028234e38:  # (the factor of exp2, in single precision)
         raise BLASError(StatusCode.kInvalidValue)
     return scale
 
@@ -414,6 +414,8 @@ def attention(Q, K, V, Y, scale=None, key_lengths=None, key_mask=None, queue=Non
     may hold anything. A query with no key gets zeros. Any strides that are multiples of 8 elements, over 16-byte aligned
     addresses, with a head's values contiguous; Q, K, V and the mask may be shared by the batch (expanded). Y must not overlap the
     inputs."""
+    if scale is not None:
+        scale = float(scale)  # (its value belongs to the key below, not the object)
     key = (Q.dtype, K.dtype, V.dtype, Y.dtype, Q.device, K.device, V.device, Y.device, Q.shape, K.shape, V.shape, Y.shape, Q.stride(), K.stride(),
            V.stride(), Y.stride(), scale,
            None if key_mask is None else (key_mask.dtype, key_mask.device, key_mask.shape, key_mask.stride()))
@@ -457,6 +459,8 @@ def paged_attention(Q, K_pages, V_pages, page_table, lengths, Y, scale=None, que
     V_pages (pages, page_size, kv_heads, size; any strides as in ``attention``). Position i of sequence b lies in page
     page_table[b][i // page_size] (int32) at i % page_size; lengths[b] (int32) positions count, the new token's among them if
     ``paged_append`` has put it there. Table entries beyond a sequence's length may be anything."""
+    if scale is not None:
+        scale = float(scale)  # (its value belongs to the key below, not the object)
     key = (Q.dtype, K_pages.dtype, V_pages.dtype, Y.dtype, page_table.dtype, Q.device, K_pages.device, V_pages.device, Y.device,
            page_table.device, Q.shape, K_pages.shape, V_pages.shape, Y.shape, page_table.shape, Q.stride(), K_pages.stride(), V_pages.stride(),
            Y.stride(), page_table.stride(), scale)
@@ -484,7 +488,8 @@ def _append_plan(K, V, K_pages, V_pages, page_table):
 
 def paged_append(K, V, K_pages, V_pages, page_table, positions, sequences=None, queue=None, event=None):
     """New keys and values K and V (tokens, kv_heads, size) into a paged cache (see ``paged_attention``): token i to position
-    positions[i] of sequence sequences[i] (both int32; without ``sequences``, of sequence i). The rest of the cache stays as it is."""
+    positions[i] of sequence sequences[i] (both int32; without ``sequences``, of sequence i). A position below 0 marks a token that is padding and goes nowhere. The rest
+    of the cache stays as it is."""
     key = (K.dtype, V.dtype, K_pages.dtype, V_pages.dtype, page_table.dtype, K.device, V.device, K_pages.device, V_pages.device,
            page_table.device, K.shape, V.shape, K_pages.shape, V_pages.shape, page_table.shape, K.stride(), V.stride(), K_pages.stride(),
            V_pages.stride(), page_table.stride())

@@ -295,7 +295,7 @@ size_t dlf_b200_gemm_int8_workspace_bytes(size_t m, size_t n, size_t k, const si
  *
  * Lengths below 0 count as 0 and those beyond the keys there are as all of them; keys on a page that is none of the
  * num_pages do not count, and tokens for a position or page that does not exist are left out. Such lengths, positions and pages are
- * reported by bit 1 of dlf_b200_device_status (a length below 0 is not); nothing outside the tensors is read or written. */
+ * reported by bit 1 of dlf_b200_device_status (a length or a position below 0, as of padding, is not); nothing outside the tensors is read or written. */
 typedef struct {
     int dtype;
     float scale;
