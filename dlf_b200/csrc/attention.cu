@@ -9,6 +9,7 @@
 #include "../../include/dlf_b200.h"
 #include "attention_decode.cuh"
 #include "attention_plan.h"
+#include "attention_short.cuh"
 #include "attention_tiles.cuh"
 #include "host.cuh"
 
@@ -36,6 +37,7 @@ int attention_limits() {
                    attention_decode_kernel<BF16, DP, KEYS_PAGES_16, 2, true>, attention_decode_kernel<BF16, DP, KEYS_ANY, 2, true>,
                    attention_decode_kernel<BF16, DP, KEYS_ANY, 2, false>})
         CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(DP, 2)));
+    CUDA_TRY(cudaFuncSetAttribute(attention_short_kernel<BF16, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, short_smem(DP, kTileKeys, 2)));
     CUDA_TRY(cudaFuncSetAttribute(attention_tiles_kernel<BF16, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, tiles_smem(DP)));
     return kSuccess;
 }
@@ -110,7 +112,7 @@ template <bool BF16, int DP>
 int tiles_launch(const TilesParams& p, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& y, cudaStream_t stream) {
     CUDA_TRY(launch_dependent(attention_tiles_kernel<BF16, DP>, static_cast<unsigned>(p.ctas), kTilesThreads, tiles_smem(DP), stream, p, q, k, v, y));
     count_launch();
-    if (p.keys > kTileKeys && p.ctas > 1) {
+    if (p.ctas > 1) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(p.ctas - 1), 256 / kTilesJoinRows, 1);
         cfg.blockDim = dim3(128, 1, 1);
@@ -123,6 +125,20 @@ int tiles_launch(const TilesParams& p, const CUtensorMap& q, const CUtensorMap& 
         CUDA_TRY(cudaLaunchKernelEx(&cfg, attention_tiles_join_kernel<BF16>, p));
         count_launch();
     }
+    CUDA_TRY(cudaGetLastError());
+    return kSuccess;
+}
+
+template <bool BF16, int DP>
+int short_launch(ShortParams& p, int num_sms, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const CUtensorMap& y, cudaStream_t stream) {
+    // The next tile's queries in a buffer of their own, unless that leaves one block to an SM (heads of 128 over more than 80 keys:
+    // 16 x 4096 queries over 112, 8 heads, 84 us with one buffer and two blocks, 92 with two and one); not for a fourth block (heads
+    // of 64 over more than 80: 35.6 us over 96 keys with three blocks of two buffers, 38.4 with four of one).
+    auto per_sm_with = [&](int buffers) { return std::min(short_ctas_per_sm(DP), 228 * 1024 / (short_smem(DP, p.key_rows, buffers) + 1280)); };
+    p.buffers = per_sm_with(2) < 2 ? 1 : 2;
+    const int per_sm = per_sm_with(p.buffers), smem = short_smem(DP, p.key_rows, p.buffers);
+    CUDA_TRY(launch_dependent(attention_short_kernel<BF16, DP>, static_cast<unsigned>(std::min(p.tiles, num_sms * per_sm)), kShortThreads, smem, stream, p, q, k, v, y));
+    count_launch();
     CUDA_TRY(cudaGetLastError());
     return kSuccess;
 }
@@ -213,6 +229,44 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
         p.status = dev.status;
         return decode_any(p, bf16, s);
     }
+    const bool inject = (tuning_bits() & 0x10000000u) != 0 && items == 1;
+    const long long wait_limit = inject ? (1ll << 21) : (1ll << 32);
+    const bool single = keys <= kTileKeys;
+    const unsigned key_rows = single ? static_cast<unsigned>((keys + 15) / 16 * 16) : kTileKeys;
+    CUtensorMap mq, mk, mv, my;
+    rc = encode_heads(dev, &mq, q, size, queries, heads, batch, q_strides[1], q_strides[2], q_strides[0], 128);
+    if (rc == kSuccess) rc = encode_heads(dev, &mk, k, size, keys, kv_heads, batch, k_strides[1], k_strides[2], k_strides[0], key_rows);
+    if (rc == kSuccess) rc = encode_heads(dev, &mv, v, size, keys, kv_heads, batch, v_strides[1], v_strides[2], v_strides[0], key_rows);
+    if (rc == kSuccess) rc = encode_heads(dev, &my, y, size, queries, heads, batch, y_strides[1], y_strides[2], y_strides[0], 32, !single && size <= 64 ? 32 : 64);
+    if (rc != kSuccess) return rc;
+    if (single) {
+        const long long q_tiles = static_cast<long long>((queries + 127) / 128), tiles = q_tiles * static_cast<long long>(heads) * static_cast<long long>(batch);
+        if (tiles > INT_MAX) return kInvalidDimension;
+        ShortParams p{};
+        p.batch = static_cast<int>(batch);
+        p.queries = static_cast<int>(queries);
+        p.keys = static_cast<int>(keys);
+        p.heads = static_cast<int>(heads);
+        p.group = static_cast<int>(group);
+        p.size = static_cast<int>(size);
+        p.lengths = key_lengths;
+        p.mask = key_mask;
+        p.mask_sb = static_cast<long long>(key_mask_ld);
+        p.q_tiles = static_cast<int>(q_tiles);
+        p.tiles = static_cast<int>(tiles);
+        p.key_rows = static_cast<int>(key_rows);
+        p.k_batched = k_strides[0] != 0;
+        p.v_batched = v_strides[0] != 0;
+        p.q_batched = q_strides[0] != 0;
+        p.c = c;
+        p.y = static_cast<char*>(y);
+        p.y_sb = y_strides[0], p.y_st = y_strides[1], p.y_sh = y_strides[2];
+        p.status = dev.status;
+        p.wait_limit = wait_limit;
+        p.withhold = inject ? 1 : 0;
+        if (size <= 64) return bf16 ? short_launch<true, 64>(p, dev.num_sms, mq, mk, mv, my, s) : short_launch<false, 64>(p, dev.num_sms, mq, mk, mv, my, s);
+        return bf16 ? short_launch<true, 128>(p, dev.num_sms, mq, mk, mv, my, s) : short_launch<false, 128>(p, dev.num_sms, mq, mk, mv, my, s);
+    }
     TilesParams p{};
     p.batch = static_cast<int>(batch);
     p.queries = static_cast<int>(queries);
@@ -234,15 +288,8 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     p.v_batched = v_strides[0] != 0;
     p.c = c;
     p.status = dev.status;
-    const bool inject = (tuning_bits() & 0x10000000u) != 0 && units == 1;
-    p.wait_limit = inject ? (1ll << 21) : (1ll << 32);
+    p.wait_limit = wait_limit;
     p.withhold = inject ? 1 : 0;
-    CUtensorMap mq, mk, mv, my;
-    rc = encode_heads(dev, &mq, q, size, queries, heads, batch, q_strides[1], q_strides[2], q_strides[0], 128);
-    if (rc == kSuccess) rc = encode_heads(dev, &mk, k, size, keys, kv_heads, batch, k_strides[1], k_strides[2], k_strides[0], 128);
-    if (rc == kSuccess) rc = encode_heads(dev, &mv, v, size, keys, kv_heads, batch, v_strides[1], v_strides[2], v_strides[0], 128);
-    if (rc == kSuccess) rc = encode_heads(dev, &my, y, size, queries, heads, batch, y_strides[1], y_strides[2], y_strides[0], 32, size <= 64 ? 32 : 64);
-    if (rc != kSuccess) return rc;
     if (size <= 64) return bf16 ? tiles_launch<true, 64>(p, mq, mk, mv, my, s) : tiles_launch<false, 64>(p, mq, mk, mv, my, s);
     return bf16 ? tiles_launch<true, 128>(p, mq, mk, mv, my, s) : tiles_launch<false, 128>(p, mq, mk, mv, my, s);
 }

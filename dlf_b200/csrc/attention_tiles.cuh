@@ -1,4 +1,4 @@
-// Attention of many query rows: two tiles of 128 queries per CTA against tiles of 128 keys, on the tensor cores.
+// Attention of many query rows over more than 128 keys: two tiles of 128 queries per CTA against tiles of 128 keys, on the tensor cores.
 //
 //     S = Q K^T,  p = exp2(c S - c m),  O = sum over key tiles of P V,  y = O / sum p      (c = scale * log2 e)
 //

@@ -287,6 +287,45 @@ def test_attention_of_many_queries(dtype, padding, lq, lk, h, hk, d):
     _check_attention(3, lq, lk, h, hk, d, dtype, padding)
 
 
+@pytest.mark.parametrize("d", [40, 64, 96, 128])
+@pytest.mark.parametrize("lk", [1, 16, 17, 64, 77, 80, 81, 96, 97, 112, 128])
+def test_attention_of_many_queries_over_few_keys(d, lk):
+    """One tile of keys: sizes on either side of its steps, entries without keys between others."""
+    for i, padding in enumerate(("none", "lengths", "mask", "both")):
+        _check_attention(4, 33 + 50 * i, lk, 4, 2, d, HALF[i % 2], padding, seed=lk)
+        _check_attention(3, 150, lk, 3, 1, d, HALF[1 - i % 2], padding, layout="heads first")
+
+
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("lk", [60, 120])
+def test_attention_over_few_keys_that_the_batch_shares(d, lk):
+    _check_attention(5, 140, lk, 4, 2, d, torch.float16, "lengths", shared=True)
+    _check_attention(5, 140, lk, 4, 4, d, torch.bfloat16, "one mask", shared=True)
+
+
+@pytest.mark.parametrize("d,lk", [(64, 77), (64, 128), (128, 50), (128, 128)])
+def test_attention_over_few_keys_with_many_tiles_a_block(d, lk):
+    """More tiles of queries than blocks, so that a block goes on to other queries, heads and entries, some of them without keys."""
+    _check_attention(9, 600, lk, 24, 8, d, torch.bfloat16, "lengths")
+    _check_attention(6, 700, lk, 20, 20, d, torch.float16, "both")
+
+
+def test_attention_wait_that_runs_out_is_reported_over_many_keys():
+    q, k = (torch.ones(1, n, 1, 64, dtype=torch.float16, device="cuda") for n in (200, 250))
+    y = torch.empty_like(q)
+    gdnn.attention(q, k, k, y)
+    L = dlf_b200.lib()
+    try:
+        L.dlf_b200_set_tuning(0, 0x10000000)
+        gdnn.attention(q, k, k, torch.empty_like(q))
+        assert dlf_b200.device_status() & 1
+    finally:
+        L.dlf_b200_set_tuning(0, 0)
+    y = torch.empty_like(q)
+    gdnn.attention(q, k, k, y)
+    assert bool((y == 1).all()) and dlf_b200.device_status() == 0
+
+
 @pytest.mark.parametrize("d", [8, 16, 40, 72, 80, 96, 120])
 @pytest.mark.parametrize("lq", [1, 40])
 def test_attention_head_sizes(d, lq):
