@@ -147,7 +147,9 @@ int short_launch(ShortParams& p, int num_sms, const CUtensorMap& q, const CUtens
 // there are rows, the other one as if every head had 128 queries at least; with 32 entries of 1500 keys and 8 heads (us, this
 // kernel and the other): heads of 64 24 and 47 (16 queries), 33 and 47 (32), 53 and 48 (64); heads of 128 45 and 59 (16), 73 and
 // 60 (32). 32 query heads on one kv head, 1 query: 13 and 128.
-bool few_rows(size_t queries, size_t size) { return queries <= (size <= 64 ? 32 : 16); }
+// Over up to 128 keys the other one is attention_short_kernel, and 8 queries are few: 256 entries of 77 keys, 8 heads (us), heads of
+// 64 17 and 19 (8 queries), 23 and 19 (16), 44 and 19 (32); heads of 128 25 and 30 (8), 40 and 31 (16).
+bool few_rows(size_t queries, size_t keys, size_t size) { return queries <= (keys <= kTileKeys ? 8 : size <= 64 ? 32 : 16); }
 
 int head_args(int dtype, size_t heads, size_t kv_heads, size_t size) {
     if (dtype != DLF_B200_HALF && dtype != DLF_B200_BFLOAT16) return kNotImplemented;
@@ -163,7 +165,7 @@ extern "C" {
 size_t dlf_b200_attention_workspace_bytes(size_t batch, size_t queries, size_t keys, size_t heads, size_t kv_heads, size_t size) {
     (void)batch;
     if (kv_heads == 0 || heads % kv_heads != 0) return 0;
-    return few_rows(queries, size) ? decode_workspace(size) : tiles_workspace(keys, size);
+    return few_rows(queries, keys, size) ? decode_workspace(size) : tiles_workspace(keys, size);
 }
 
 int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -187,7 +189,7 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     if ((keys > 1 && (k_strides[1] == 0 || v_strides[1] == 0)) || (kv_heads > 1 && (k_strides[2] == 0 || v_strides[2] == 0))) return kInvalidLeadDimB;
     const bool bf16 = dtype == DLF_B200_BFLOAT16;
     const size_t group = heads / kv_heads;
-    const bool few = few_rows(queries, size);
+    const bool few = few_rows(queries, keys, size);
     const size_t need = dlf_b200_attention_workspace_bytes(batch, queries, keys, heads, kv_heads, size);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return kInsufficientMemoryTemp;
     const long long items = static_cast<long long>((queries + 255) / 256) * static_cast<long long>(heads) * static_cast<long long>(batch);

@@ -261,7 +261,7 @@ def _check_attention(b, lq, lk, h, hk, d, dtype, padding="none", garbage=True, s
         k[~keep], v[~keep] = math.nan, math.inf
     kx, vx = (k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1)) if shared else (k, v)
     gdnn.attention(q, kx, vx, y, scale=scale, key_lengths=lengths, key_mask=mask)
-    few = lq <= (32 if d <= 64 else 16)  # the kernel that keeps P in two parts
+    few = lq <= (8 if lk <= 128 else 32 if d <= 64 else 16)  # the kernel that keeps P in two parts; the others round it once, half a step each
     for i in range(b):
         want, a, e = _attention_want(q[i], kx[i], vx[i], keep[i], scale or 1 / math.sqrt(d))
         _check_rows(y[i], want, a, e, dtype, _half_step(dtype) ** 2 if few else _half_step(dtype))
@@ -292,6 +292,7 @@ def test_attention_of_many_queries(dtype, padding, lq, lk, h, hk, d):
 def test_attention_of_many_queries_over_few_keys(d, lk):
     """One tile of keys: sizes on either side of its steps, entries without keys between others."""
     for i, padding in enumerate(("none", "lengths", "mask", "both")):
+        _check_attention(3, (8, 9, 20, 32)[i], lk, 4, 1, d, HALF[i % 2], padding, seed=lk)
         _check_attention(4, 33 + 50 * i, lk, 4, 2, d, HALF[i % 2], padding, seed=lk)
         _check_attention(3, 150, lk, 3, 1, d, HALF[1 - i % 2], padding, layout="heads first")
 
