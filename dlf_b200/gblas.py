@@ -330,7 +330,19 @@ def _gemm(layout, a_transpose, b_transpose, m, n, k, alpha, a, a_ld, b, b_ld, be
 # ---------------------------------------------------------------------------------------------
 # Products in 8-bit integers. The reference has no such routine; names and argument order follow gemm.
 
+class _Plans(dict):
+    """What is known of a call from its tensors' types, devices, shapes and strides - that they fit together, and the library's arguments
+    made of them - so that a call like an earlier one only looks this up. Started anew when it has grown."""
+
+    def keep(self, key, plan):
+        if len(self) >= 512:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
 _INT8_WORKSPACES = {}
+_INT8_NEEDS = _Plans()
 
 
 def _operator_stream(queue, device):
@@ -425,7 +437,10 @@ def _gemm_int8(prec, m, n, k, a, a_ld, a_scales, b, b_ld, b_scales, bias, activa
     handle = _operator_stream(queue, device)
     ws, entry, need = None, None, 0
     if (a | b) & 15 or (a_ld | b_ld) & 15:  # operands that may have to be copied first (not those of one line)
-        need = L.dlf_b200_gemm_int8_workspace_bytes(m, n, k, a, a_ld, b, b_ld)
+        key = (m, n, k, a & 15, a_ld, b & 15, b_ld)  # (all that it depends on)
+        need = _INT8_NEEDS.get(key)
+        if need is None:
+            need = _INT8_NEEDS.keep(key, L.dlf_b200_gemm_int8_workspace_bytes(m, n, k, a, a_ld, b, b_ld))
         if need:
             ws, entry = _operator_scratch(_INT8_WORKSPACES, need, device, queue, handle)
     with entry.lock if entry is not None else _NO_LOCK:
@@ -439,17 +454,6 @@ def _gemm_int8(prec, m, n, k, a, a_ld, a_scales, b, b_ld, b_scales, bias, activa
         if event is not None:
             event.end.record(s)
     _check(rc)
-
-
-class _Plans(dict):
-    """What is known of a call from its tensors' types, devices, shapes and strides - that they fit together, and the library's arguments
-    made of them - so that a call like an earlier one only looks this up. Started anew when it has grown."""
-
-    def keep(self, key, plan):
-        if len(self) >= 512:
-            self.clear()
-        self[key] = plan
-        return plan
 
 
 def gemmStridedBatched(layout, a_transpose, b_transpose, m, n, k, alpha, a_buffer, a_offset, a_ld,
