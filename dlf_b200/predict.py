@@ -122,6 +122,23 @@ class Graph:
         self.outputs.append(value)
         return value
 
+    def copy(self):
+        """The same graph in nodes and values of its own, for passes that are one list's alone; graph inputs and initializers
+        are shared."""
+        g, made = Graph(), {}
+        for node in self.nodes:
+            n = g.append(node.kind)
+            for v in node.outputs:
+                w = n.addOutput(v.name)
+                w.dtype, w.dims, w.initializer = v.dtype, v.dims, v.initializer
+                made[id(v)] = w
+        for node, n in zip(self.nodes, g.nodes):  # (behind all outputs: nodes need not be in order)
+            n.inputs = [made.get(id(v), v) for v in node.inputs]
+            n.attrs = {name: made.get(id(v), v) for name, v in node.attrs.items()}
+        g.inputs = list(self.inputs)
+        g.outputs = [made.get(id(v), v) for v in self.outputs]
+        return g
+
     # -- what the optimizer passes need ------------------------------------------------------
 
     def uses(self, value):
@@ -715,6 +732,8 @@ class Predictor:
         optimize(graph)
         self._int8 = bool(int8)
         if self._int8:
+            # only this list's products clamp by themselves: the caller's graph keeps its Relu nodes for other lists
+            graph = graph.copy()
             fuse_relu_into_int8_products(graph)
         left = unsupported_nodes(graph)
         if left:
@@ -885,6 +904,8 @@ class Predictor:
                 raise NotImplementedError("Attention: float16 or bfloat16 and heads of a multiple of 8 values up to 128")
             scale = float(n.get("scale", 0.0)) or None
             return AttentionOp(Q, K, V, Y, self._alloc(n.input(6)), scale)
+        if k in ("Gemm", "MatMul") and n.get("relu"):  # (fuse_relu_into_int8_products has been here)
+            raise NotImplementedError("%s with a Relu: 8-bit integers only" % k)
         if k == "Gemm":
             A, B, C = self._alloc(n.input(0)), self._alloc(n.input(1)), self._alloc(n.input(2))
             return GemmOp(A, B, C, self._alloc(n.output(0)), n.get("alpha", 1.0), n.get("beta", 1.0),

@@ -369,3 +369,72 @@ def test_streams_of_another_device_are_refused():
 
     _refused(StatusCode.kInvalidValue, gblas._operator_stream, Queue(), torch.device("cuda", 0))
     assert gblas._operator_stream(Queue(), torch.device("cuda", 1)) == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# one graph, several lists
+
+
+def _gemm_relu_graph():
+    g = predict.Graph()
+    n = g.append("Gemm")
+    n.addInput(g.addInput("a", predict.DataType.FLOAT, (4, 8)))
+    n.addInput(g.addInitializer("w", np.ones((8, 6), np.float32)))
+    r = g.append("Relu")
+    r.addInput(n.addOutput("y"))
+    m = g.append("MatMul")
+    m.addInput(r.addOutput("r"))
+    m.addInput(g.addInitializer("w2", np.ones((6, 3), np.float32)))
+    g.addOutput(m.addOutput("z"))
+    return g
+
+
+def _rounded_on_the_host(monkeypatch):
+    """Lists of 8-bit products without a device: the weights are not rounded, only passed on."""
+    monkeypatch.setattr(predict.linalg, "quantize", lambda W, *out: (W, torch.ones(W.shape[0])))
+
+
+def test_a_list_of_8_bit_products_leaves_its_graph_as_it_was(monkeypatch):
+    _rounded_on_the_host(monkeypatch)
+    g = _gemm_relu_graph()
+    for _ in range(2):
+        with pytest.raises(NotImplementedError):  # a Relu behind a product in floating point is outside the library's path
+            predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False)
+        p = predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False, int8=True)
+        assert [(type(op).__name__, op.relu) for op in p.operators] == [("Int8ProductOp", True), ("Int8ProductOp", False)]
+        assert p.operators[0].Y is p.operators[1].A
+        assert [n.kind for n in g.nodes] == ["Gemm", "Relu", "MatMul"] and not any(n.get("relu") for n in g.nodes)
+
+
+def test_a_copied_graph_shares_nothing_that_a_pass_changes():
+    g = predict.Graph()
+    x, w = g.addInput("x", predict.DataType.FLOAT, (1, 8, 6, 6)), g.addInitializer("w", np.ones((8, 8, 1, 1), np.float32))
+    values = [x]
+    for name in ("a", "b"):
+        n = g.append("Conv", kernel_shape=(1, 1))
+        n.addInput(values[-1])
+        n.addInput(w)
+        values.append(n.addOutput(name))
+    add = g.append("Add")
+    add.addInput(values[2])
+    add.addInput(values[1])
+    g.addOutput(add.addOutput("y"))
+    predict.infer_shapes(g)
+    predict.optimize(g)
+    assert g.nodes[1].attrs["residual"] is values[1]
+    c = g.copy()
+    assert c.inputs == g.inputs and c.inputs is not g.inputs
+    a, b = c.nodes
+    assert a.output(0) is not values[1] and a.output(0).dims == values[1].dims and a.output(0).node is a
+    assert b.input(0) is a.output(0) and b.attrs["residual"] is a.output(0) and c.outputs == [b.output(0)]
+    assert a.input(0) is x and a.input(1) is w
+    assert [type(op).__name__ for op in predict.Predictor(c, torch.float32, device="cpu").operators] == ["ConvOp", "ConvOp"]
+
+
+def test_a_graph_marked_for_8_bit_products_is_refused_in_floating_point(monkeypatch):
+    _rounded_on_the_host(monkeypatch)
+    g = predict.infer_shapes(_gemm_relu_graph())
+    assert predict.fuse_relu_into_int8_products(g)
+    with pytest.raises(NotImplementedError):
+        predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False)
+    assert predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False, int8=True).operators[0].relu
