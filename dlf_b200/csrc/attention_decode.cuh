@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
 
     PlanWalk walk(decode_lengths(p), p.kv_heads * p.row_blocks, p.ctas, p.least);
     const int chunks = p.size / 8;
-    const float c = p.c, limit = 8.0f / c;
+    // (finite however small the scale: -infinity + infinity would never be exceeded)
+    const float c = p.c, limit = fminf(8.0f / c, 3.402823466e38f);
     bool bad_page = false;
 
     for (; walk.more(); walk.next()) {

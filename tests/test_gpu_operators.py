@@ -360,6 +360,23 @@ def test_attention_scores_that_grow_and_scales(lq, d):
             _check_rows(y[0], want, a, e, dtype, _half_step(dtype) if lq > 32 else _half_step(dtype) ** 2)
 
 
+@pytest.mark.parametrize("scale", [1.7e-38, 1e-38, 1e-44])
+def test_attention_scales_that_leave_nothing_between_the_keys(scale):
+    """The mean of the kept values, whichever kernel takes the call."""
+    for dtype in HALF:
+        for lq, lk in ((1, 300), (1, 3000), (20, 300), (200, 300), (200, 100)):
+            _check_attention(2, lq, lk, 4, 2, 64, dtype, "lengths", scale=scale)
+        g = torch.Generator(device="cuda").manual_seed(1)
+        table, kp, vp = _cache(g, 2, 100, 16, 2, 64, dtype)
+        q = torch.randn(2, 4, 64, generator=g, device="cuda").to(dtype)
+        y = torch.empty_like(q)
+        gdnn.paged_attention(q, kp, vp, table, torch.tensor([100, 33], dtype=torch.int32, device="cuda"), y, scale=scale)
+        for i, n in enumerate((100, 33)):
+            k, v = (t[table[i].long()].reshape(-1, 2, 64)[:n] for t in (kp, vp))
+            want, a, e = _attention_want(q[i:i + 1], k, v, torch.ones(n, dtype=torch.bool, device="cuda"), scale)
+            _check_rows(y[i:i + 1], want, a, e, dtype, _half_step(dtype) ** 2)
+
+
 @pytest.mark.parametrize("b,lq,lk,h,hk,d", [(1, 256, 40000, 1, 1, 64), (1, 40, 9000, 2, 1, 128), (2, 300, 5000, 3, 1, 80), (1, 1, 60000, 4, 1, 128)])
 def test_attention_over_many_keys_is_cut_and_joined(b, lq, lk, h, hk, d):
     _check_attention(b, lq, lk, h, hk, d, torch.bfloat16, "lengths")
