@@ -1,7 +1,11 @@
 // Attention of few query rows over many keys: one new token (or a few) of each sequence over a paged cache or over an
 // encoder's states.
 //
-//     y_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp2(c q_r.k_j - m_r),  c = scale * log2(e),  m_r the largest so far
+//     y_r = sum_j p_rj v_j / sum_j p_rj,   p_rj = exp2(c (q_r.k_j - m_r)),  c = scale * log2(e),  m_r the largest so far
+//
+// The difference is taken before it is multiplied: of c s - c m in one fused step (c m rounded) the rounding of c m would be
+// left, which for scores beyond 2^30 / c is more than exp2's range. Parts of a sequence are joined by the same rule, so m itself is
+// what they leave beside their sums.
 //
 // HBM-bound: the keys and values of a kv head are read once for up to 16 query rows (the query heads that share it), so
 // what counts is how many bytes are in flight and how few instructions a key costs. A block has four warps; of a unit of 64
@@ -50,6 +54,8 @@ struct DecodeParams {
 // where a sequence's keys lie: one after the other; in pages of a multiple of 16 tokens (a step's 16 keys lie in one page); in
 // pages of any size, or under a mask (every key by itself)
 enum : int { KEYS_PLAIN = 0, KEYS_PAGES_16 = 1, KEYS_ANY = 2 };
+
+constexpr float kLowest = -3.402823466e38f;  // below every score that counts; finite, so that differences from it are none of inf - inf
 
 constexpr int kDecodeUnit = 64;  // keys
 constexpr int kDecodeThreads = 128;
@@ -143,8 +149,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
 
     PlanWalk walk(decode_lengths(p), p.kv_heads * p.row_blocks, p.ctas, p.least);
     const int chunks = p.size / 8;
-    // (finite however small the scale: -infinity + infinity would never be exceeded)
-    const float c = p.c, limit = fminf(8.0f / c, 3.402823466e38f);
+    const float c = p.c;
     bool bad_page = false;
 
     for (; walk.more(); walk.next()) {
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int x = 0; x < DP / 16; ++x) o[nb][x][0] = o[nb][x][1] = o[nb][x][2] = o[nb][x][3] = 0.0f;
-            m[nb][0] = m[nb][1] = -INFINITY;
+            m[nb][0] = m[nb][1] = kLowest;
             l[nb][0] = l[nb][1] = 0.0f;
         }
         // ---------------------------------------------------------------- keys
@@ -312,7 +317,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) grew |= fmaxf(sc[nb][r], sc[nb][2 + r]) > m[nb][r] + limit;
+                        for (int r = 0; r < 2; ++r) grew |= fmaxf(sc[nb][r] - m[nb][r], sc[nb][2 + r] - m[nb][r]) * c > 8.0f;
                     if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb)
@@ -338,9 +343,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
                         float e[4];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            const float mc = m[nb][r] == -INFINITY ? 0.0f : m[nb][r] * c;
-                            e[r] = ptx::exp2_approx(fmaf(sc[nb][r], c, -mc));
-                            e[2 + r] = ptx::exp2_approx(fmaf(sc[nb][2 + r], c, -mc));
+                            e[r] = ptx::exp2_approx((sc[nb][r] - m[nb][r]) * c);
+                            e[2 + r] = ptx::exp2_approx((sc[nb][2 + r] - m[nb][r]) * c);
                             l[nb][r] += e[r] + e[2 + r];
                         }
 #pragma unroll
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
         }
         // ---------------------------------------------------------------- the four warps' results
         ptx::cp_async_wait<0>();
-        __syncthreads();  // the rings are free: [warp][16 rows][DP + 4] sums, then [warp][16][2] maximum (times c) and sum
+        __syncthreads();  // the rings are free: [warp][16 rows][DP + 4] sums, then [warp][16][2] maximum and sum
         float* sums = reinterpret_cast<float*>(smem_raw);
         float* stat = sums + kDecodeWarps * 16 * (DP + 4);
 #pragma unroll
@@ -386,7 +390,7 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
                     to[16 * x + 8] = o[nb][x][2 + r];
                 }
                 if (g == 0) {
-                    stat[(warp * 16 + row) * 2] = m[nb][r] * c;
+                    stat[(warp * 16 + row) * 2] = m[nb][r];
                     stat[(warp * 16 + row) * 2 + 1] = s;
                 }
             }
@@ -394,12 +398,12 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
         float* part = p.parts + static_cast<long long>(walk.slot()) * decode_slot(p.size);
         for (int id = threadIdx.x; id < rows * chunks; id += kDecodeThreads) {
             const int r = id / chunks, ch = id - r * chunks;
-            float mm = -INFINITY, ll = 0.0f, f[kDecodeWarps], acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            float mm = kLowest, ll = 0.0f, f[kDecodeWarps], acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < kDecodeWarps; ++w) mm = fmaxf(mm, stat[(w * 16 + r) * 2]);
 #pragma unroll
             for (int w = 0; w < kDecodeWarps; ++w) {
-                f[w] = mm == -INFINITY ? 0.0f : ptx::exp2_approx(stat[(w * 16 + r) * 2] - mm);
+                f[w] = ptx::exp2_approx((stat[(w * 16 + r) * 2] - mm) * c);
                 ll += f[w] * stat[(w * 16 + r) * 2 + 1];
                 const float* from = sums + (w * 16 + r) * (DP + 4) + ch * 8;
 #pragma unroll
@@ -450,14 +454,14 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     for (int id = threadIdx.x; id < rows * chunks; id += blockDim.x) {
         const int r = id / chunks, ch = id - r * chunks;
         // a running maximum, so that a part's statistics and values are asked for together
-        float mm = -INFINITY, ll = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+        float mm = kLowest, ll = 0.0f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int c = c0; c <= c1; ++c) {
             const float* part = c == c0 ? first_part : p.parts + 2ll * c * slot_floats;
             const float4 x = *reinterpret_cast<const float4*>(part + r * p.size + ch * 4);
             const float2 st = *reinterpret_cast<const float2*>(part + 16 * p.size + 2 * r);
-            const float m_new = fmaxf(mm, st.x), base = m_new == -INFINITY ? 0.0f : m_new;
-            const float f = ptx::exp2_approx(mm - base), g = ptx::exp2_approx(st.x - base);
+            const float m_new = fmaxf(mm, st.x);
+            const float f = ptx::exp2_approx((mm - m_new) * p.c), g = ptx::exp2_approx((st.x - m_new) * p.c);
             mm = m_new;
             ll = ll * f + st.y * g;
             acc[0] = acc[0] * f + x.x * g;

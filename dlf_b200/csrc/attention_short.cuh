@@ -1,6 +1,6 @@
 // Attention of many query rows over few keys: one tile of up to 128 keys (an image's or a decoder's positions over a short text).
 //
-//     S = Q K^T,  p = exp2(c S - c m),  O = P V,  y = O / sum p      (c = scale * log2 e, m the largest score of the row)
+//     S = Q K^T,  p = exp2(c (S - m)),  O = P V,  y = O / sum p      (c = scale * log2 e, m the largest score of the row)
 //
 // All the keys are there at once, so there is no recurrence and nothing is cut. What is left is a chain for each tile of 128 queries -
 // load, S, softmax, P V, store - that no unit fills, so what counts is how many tiles an SM has in flight, each at another place of its
@@ -253,8 +253,8 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas_per_sm(DP))
                 }
             }
             mx = ptx::max_of(mx, mx1, mx1);
-            const float mc = mx == -INFINITY ? 0.0f : mx * c;
-            const uint64_t c2 = ptx::pair_of(c, c), mc2 = ptx::pair_of(-mc, -mc);
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            const uint64_t c2 = ptx::pair_of(c, c), base2 = ptx::pair_of(-base, -base);
             uint64_t l2 = ptx::pair_of(0.0f, 0.0f), l3 = l2;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas_per_sm(DP))
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
                     float a, b;
-                    uint64_t s = ptx::fma_pair(ptx::pair_of(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), c2, mc2);
+                    uint64_t s = ptx::mul_pair(ptx::add_pair(ptx::pair_of(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), base2), c2);
                     ptx::of_pair(s, a, b);
                     a = ptx::exp2_approx(a);
                     b = ptx::exp2_approx(b);

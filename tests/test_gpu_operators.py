@@ -377,6 +377,33 @@ def test_attention_scales_that_leave_nothing_between_the_keys(scale):
             _check_rows(y[i:i + 1], want, a, e, dtype, _half_step(dtype) ** 2)
 
 
+@pytest.mark.parametrize("lq,lk", [(1, 300), (20, 300), (200, 300), (200, 100), (1, 60000), (40, 9000)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_scores_beyond_the_range_of_exp2(lq, lk, d):
+    """Scores whose distance, and whose own rounding once they are scaled, is more than exp2 can take: what counts are the keys with
+    the greatest score, equally. The scores are exact in fp32 (whole numbers below 2^8 times a power of two), so no error of theirs is left."""
+    g = torch.Generator(device="cuda").manual_seed(lk + d)
+    at = torch.randint(1, 200, (1, lk, 2, 1), generator=g, device="cuda")
+    for dtype, q_size, k_size, scale in ((torch.float16, 2.0 ** 15, 2.0 ** 8, None), (torch.bfloat16, 2.0 ** 15, 2.0 ** 8, None), (torch.bfloat16, 2.0 ** 40, 2.0 ** 30, None),
+                                         (torch.float16, 1.0, 1.0, 1e30), (torch.bfloat16, 1.0, 1.0, 1e35), (torch.float16, 2.0 ** 15, 2.0 ** 8, 1e20)):
+        q = torch.full((1, lq, 4, d), q_size, device="cuda").to(dtype)
+        q[:, 1::2], q[:, :, 1] = -q[:, 1::2], -q[:, :, 1]
+        k = (at * k_size).expand(-1, -1, -1, d).to(dtype).contiguous()
+        v = torch.randn(1, lk, 2, d, generator=g, device="cuda").to(dtype)
+        y = torch.full_like(q, 7)
+        gdnn.attention(q, k, v, y, scale=scale)
+        want, a, e = _attention_want(q[0], k[0], v[0], torch.ones(lk, dtype=torch.bool, device="cuda"), scale or 1 / math.sqrt(d))
+        _check_rows(y[0], want, a, 0 * e, dtype, _half_step(dtype))
+    table, kp, vp = _cache(g, 1, 400, 16, 2, d, torch.float16)
+    kp.copy_((torch.randint(1, 200, kp.shape[:3] + (1,), generator=g, device="cuda") * 2.0 ** 8).expand(-1, -1, -1, d))
+    q = torch.full((1, 4, d), 2.0 ** 15, dtype=torch.float16, device="cuda")
+    y = torch.full_like(q, 7)
+    gdnn.paged_attention(q, kp, vp, table, torch.tensor([400], dtype=torch.int32, device="cuda"), y)
+    k, v = (t[table[0].long()].reshape(-1, 2, d) for t in (kp, vp))
+    want, a, e = _attention_want(q, k, v, torch.ones(400, dtype=torch.bool, device="cuda"), 1 / math.sqrt(d))
+    _check_rows(y, want, a, 0 * e, torch.float16, _half_step(torch.float16) ** 2)
+
+
 @pytest.mark.parametrize("b,lq,lk,h,hk,d", [(1, 256, 40000, 1, 1, 64), (1, 40, 9000, 2, 1, 128), (2, 300, 5000, 3, 1, 80), (1, 1, 60000, 4, 1, 128)])
 def test_attention_over_many_keys_is_cut_and_joined(b, lq, lk, h, hk, d):
     _check_attention(b, lq, lk, h, hk, d, torch.bfloat16, "lengths")
