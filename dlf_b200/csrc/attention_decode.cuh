@@ -19,8 +19,10 @@
 //      over d has no order). No exchange, no bank conflicts.
 //   O^T += V^T P^T: V's fragments by ldmatrix.trans (lines swizzled by the key), P^T by movmatrix from S^T's accumulators.
 // The maximum of a row is moved (and O scaled) only when a score exceeds it by more than 2^8; until then a step needs no exchange
-// between lanes. p is rounded to 16 bits for the second product in two parts (its rounding and the rest), so that the result is as
-// exact as 32-bit arithmetic makes it.
+// between lanes. p is rounded to 16 bits for the second product in two parts (its rounding and the rest: 22 bits of fp16, 16 of bf16).
+// fp16 ends at 2^-24, so there p is taken times 2^7 - up to 2^15 with the growth above - and what is lost lies below 2^-32 of the
+// row's largest instead of 2^-25 (a key that outweighs the others by e^17.5 each made those of its warp nothing). The factor is the same
+// everywhere and leaves with the division by the sum.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -68,6 +70,9 @@ DLF_HD constexpr int decode_stages(int dp, int nb) { return dp <= 64 ? (nb == 1 
 DLF_HD constexpr int decode_stage_bytes(int dp) { return 16 * dp * 2 * 2; }  // a warp's 16 keys and values
 DLF_HD constexpr int decode_smem(int dp, int nb) { return kDecodeWarps * decode_stages(dp, nb) * decode_stage_bytes(dp); }
 DLF_HD constexpr int decode_slot(int size) { return 16 * (size + 2); }
+
+template <bool BF16>
+DLF_HD constexpr float decode_lift() { return BF16 ? 0.0f : 7.0f; }  // p is taken times 2 to this
 
 namespace ptx {
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {  // not valid: zeros, nothing is read
@@ -343,8 +348,8 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
                         float e[4];
 #pragma unroll
                         for (int r = 0; r < 2; ++r) {
-                            e[r] = ptx::exp2_approx((sc[nb][r] - m[nb][r]) * c);
-                            e[2 + r] = ptx::exp2_approx((sc[nb][2 + r] - m[nb][r]) * c);
+                            e[r] = ptx::exp2_approx(fmaf(sc[nb][r] - m[nb][r], c, decode_lift<BF16>()));
+                            e[2 + r] = ptx::exp2_approx(fmaf(sc[nb][2 + r] - m[nb][r], c, decode_lift<BF16>()));
                             l[nb][r] += e[r] + e[2 + r];
                         }
 #pragma unroll

@@ -2,6 +2,9 @@
 //
 //     S = Q K^T,  p = exp2(c (S - m)),  O = P V,  y = O / sum p      (c = scale * log2 e, m the largest score of the row)
 //
+// In fp16 p is taken times 2^15, the most that it holds (m is the largest score itself): its 11 bits then reach down to 2^-29 of the
+// largest.
+//
 // All the keys are there at once, so there is no recurrence and nothing is cut. What is left is a chain for each tile of 128 queries -
 // load, S, softmax, P V, store - that no unit fills, so what counts is how many tiles an SM has in flight, each at another place of its
 // chain: small blocks of four softmax warps (a thread a query row) and one warp for loads and products, four to an SM with heads of 64.
@@ -254,7 +257,8 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas_per_sm(DP))
             }
             mx = ptx::max_of(mx, mx1, mx1);
             const float base = mx == -INFINITY ? 0.0f : mx;
-            const uint64_t c2 = ptx::pair_of(c, c), base2 = ptx::pair_of(-base, -base);
+            constexpr float kLift = BF16 ? 0.0f : 15.0f;
+            const uint64_t c2 = ptx::pair_of(c, c), base2 = ptx::pair_of(-base, -base), lift2 = ptx::pair_of(kLift, kLift);
             uint64_t l2 = ptx::pair_of(0.0f, 0.0f), l3 = l2;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -270,7 +274,7 @@ __global__ void __launch_bounds__(kShortThreads, short_ctas_per_sm(DP))
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
                     float a, b;
-                    uint64_t s = ptx::mul_pair(ptx::add_pair(ptx::pair_of(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), base2), c2);
+                    uint64_t s = ptx::fma_pair(ptx::add_pair(ptx::pair_of(__uint_as_float(v[2 * x]), __uint_as_float(v[2 * x + 1])), base2), c2, lift2);
                     ptx::of_pair(s, a, b);
                     a = ptx::exp2_approx(a);
                     b = ptx::exp2_approx(b);

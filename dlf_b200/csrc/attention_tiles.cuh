@@ -5,7 +5,8 @@
 // The difference is taken first (attention_decode.cuh says why) where c m is beyond 2^10; below, the rounding of c m is 2^-14 at most,
 // and one fused step for c S - c m saves 3 % (2 x 4096 x 8192, 32 heads of 128: 758 us with the difference always, 735 so).
 // m is a reference near the running maximum of a row: it is moved (and O and the sum scaled) only when the maximum has grown by
-// more than 2^8 since, which exp2's range allows and which makes the pass over O rare.
+// more than 2^8 since, which exp2's range allows and which makes the pass over O rare. In fp16 p is taken times 2^7, as in
+// attention_decode.cuh.
 //
 // Bound by power with heads of 128 values (2 x 4096 x 4096, 32 heads: 458 us, 1200 TFLOP/s, the clock at 1.6 GHz; every arrangement
 // below that was tried took the same time), by latencies and the special-function unit with heads of 64 (a pair of tiles of 128 x 128
@@ -630,7 +631,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
                         factor = 1.0f;
                         less = 0.0f;
                     }
-                    const uint64_t c2 = ptx::pair_of(factor, factor), less2 = ptx::pair_of(-less, -less);
+                    const float add = decode_lift<BF16>() - less;
+                    const uint64_t c2 = ptx::pair_of(factor, factor), add2 = ptx::pair_of(add, add);
                     uint64_t l2 = ptx::pair_of(0.0f, 0.0f), l3 = l2;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {  // 32 keys each
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1)
 #pragma unroll
                         for (int x = 0; x < 16; ++x) {
                             float a, b;
-                            uint64_t s = ptx::fma_pair(ptx::pair_of(__uint_as_float(v[j][2 * x]), __uint_as_float(v[j][2 * x + 1])), c2, less2);
+                            uint64_t s = ptx::fma_pair(ptx::pair_of(__uint_as_float(v[j][2 * x]), __uint_as_float(v[j][2 * x + 1])), c2, add2);
                             ptx::of_pair(s, a, b);
                             a = ptx::exp2_approx(a);
                             b = ptx::exp2_approx(b);

@@ -404,6 +404,25 @@ def test_attention_scores_beyond_the_range_of_exp2(lq, lk, d):
     _check_rows(y, want, a, 0 * e, torch.float16, _half_step(torch.float16) ** 2)
 
 
+@pytest.mark.parametrize("b,lq,lk", [(1000, 1, 4096), (400, 20, 4096), (200, 64, 4096), (2, 200, 40000), (3, 200, 128), (3, 200, 60)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_many_keys_that_one_outweighs(b, lq, lk, d):
+    """One key is e^17.5 times as heavy as every other and has zeros for values: what is read is the others' sum. In fp16 a p below 2^-14
+    has fewer bits, a step of 2^-24: with p times 2^7 that is an error of 2^-32 of the heaviest for every key (over few keys times
+    2^15 and less than that)."""
+    for dtype in HALF:
+        for heavy in (0, lk // 3):
+            q, k, v = torch.zeros(1, 1, 1, d), torch.zeros(1, lk, 1, d), torch.ones(1, lk, 1, d)
+            q[..., 0], k[:, heavy, :, 0], v[:, heavy] = 1, 17.5, 0
+            q, k, v = (t.to(dtype).cuda() for t in (q, k, v))
+            y = torch.full((b, lq, 1, d), 7.0, dtype=dtype, device="cuda")
+            gdnn.attention(q.expand(b, lq, -1, -1).contiguous(), k.expand(b, -1, -1, -1), v.expand(b, -1, -1, -1), y, scale=1.0)
+            want, a, e = _attention_want(q[0], k[0], v[0], torch.ones(lk, dtype=torch.bool, device="cuda"), 1.0)
+            lost = lk * 2.0 ** -32 if dtype == torch.float16 else 0.0
+            want, a = (t.expand(b, lq, -1, -1) for t in (want, a + lost / 2 / _half_step(dtype)))  # (so that 2 half steps of a hold it)
+            _check_rows(y, want, a, e, dtype, _half_step(dtype))
+
+
 @pytest.mark.parametrize("b,lq,lk,h,hk,d", [(1, 256, 40000, 1, 1, 64), (1, 40, 9000, 2, 1, 128), (2, 300, 5000, 3, 1, 80), (1, 1, 60000, 4, 1, 128)])
 def test_attention_over_many_keys_is_cut_and_joined(b, lq, lk, h, hk, d):
     _check_attention(b, lq, lk, h, hk, d, torch.bfloat16, "lengths")
