@@ -443,7 +443,7 @@ template <bool BF16>
 __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ DecodeParams p) {
     const int heads = p.kv_heads * p.row_blocks;
     const int b = blockIdx.x / heads, hb = blockIdx.x - b * heads;
-    // the lengths are those the kernel before this one has read, which it lets this one start behind
+    ptx::wait_for_dependencies();  // (before the lengths too: only behind it is what earlier kernels wrote visible)
     int before, all;
     plan_sums(decode_lengths(p), b, before, all);
     const int per = plan_per(all * heads, p.ctas, p.least);
@@ -452,7 +452,6 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_consta
     const int c0 = first / per, c1 = last / per;
     const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * p.block_rows;
     const int rows = min(p.block_rows, p.tokens * p.group - row0), chunks = p.size / 4;
-    ptx::wait_for_dependencies();
     if (c0 == c1) return;
     const long long slot_floats = decode_slot(p.size);
     const float* first_part = p.parts + plan_slot(first, per) * slot_floats;

@@ -2,6 +2,7 @@
 mirror, how attention's work is shared out, the argument structures, and the operator list's new nodes."""
 import ctypes
 import os
+import re
 import shutil
 import subprocess
 
@@ -438,3 +439,15 @@ def test_a_graph_marked_for_8_bit_products_is_refused_in_floating_point(monkeypa
     with pytest.raises(NotImplementedError):
         predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False)
     assert predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False, int8=True).operators[0].relu
+
+
+@pytest.mark.parametrize("name", ["attention_decode.cuh", "attention_short.cuh", "attention_tiles.cuh", "contraction_int8.cuh", "quantize.cuh"])
+def test_kernels_read_no_device_memory_before_they_wait_for_the_kernel_before_them(name):
+    """A programmatic dependent may start while the kernel before it runs: what others wrote is visible behind the wait only."""
+    with open(os.path.join(ROOT, "dlf_b200", "csrc", name)) as f:
+        kernels = re.findall(r"__global__.*?\n}\n", f.read(), re.S)
+    assert kernels
+    for body in kernels:
+        before, wait, _ = body.partition("wait_for_dependencies();")
+        assert wait, body[:200]
+        assert not re.search(r"plan_(sums|find|sequence)\(|PlanWalk walk|p\.(lengths|table|positions|sequences|mask|sa|sb)\[|\*reinterpret_cast<const", before), before[-400:]
