@@ -63,14 +63,22 @@ bool strides_ok(std::initializer_list<size_t> s) {
 
 // (sequences of one tile of keys are never cut)
 size_t tiles_workspace(size_t keys, size_t size) { return keys > kTileKeys ? static_cast<size_t>(2 * kB200Sms) * tiles_slot(static_cast<int>(size)) * 4 : 0; }
-size_t decode_workspace(size_t size) { return static_cast<size_t>(2 * kB200Sms * decode_ctas_per_sm(static_cast<int>(size), 1)) * decode_slot(static_cast<int>(size)) * 4; }
+size_t decode_workspace(size_t size) {
+    const size_t ctas = static_cast<size_t>(kB200Sms * decode_ctas_per_sm(static_cast<int>(size), 1));
+    return ctas * (2 * decode_slot(static_cast<int>(size)) * sizeof(float) + sizeof(int4));
+}
 
 template <bool BF16, int DP, int KEYS, int NB, bool FULL>
 int decode_launch(const DecodeParams& p, cudaStream_t stream) {
     CUDA_TRY(launch_dependent(attention_decode_kernel<BF16, DP, KEYS, NB, FULL>, static_cast<unsigned>(p.ctas), kDecodeThreads, decode_smem(DP, NB), stream, p));
     count_launch();
-    CUDA_TRY(launch_dependent(attention_join_kernel<BF16>, static_cast<unsigned>(p.batch * p.kv_heads * p.row_blocks), 128u, 0, stream, p));
-    count_launch();
+    // CTAs that may have work, of which the last cuts nothing; a sequence of one unit is never cut
+    const long long units = plan_units(p.keys, kDecodeUnit), all = units * p.batch * p.kv_heads * p.row_blocks;
+    const long long busy = std::min<long long>(p.ctas, (all + p.least - 1) / p.least);
+    if (units > 1 && busy > 1) {
+        CUDA_TRY(launch_dependent(attention_join_kernel<BF16>, static_cast<unsigned>(busy - 1), 128u, 0, stream, p));
+        count_launch();
+    }
     CUDA_TRY(cudaGetLastError());
     return kSuccess;
 }
@@ -87,6 +95,7 @@ int decode_rows(DecodeParams& p, cudaStream_t stream) {
     const int rows = p.tokens * p.group;
     p.block_rows = rows <= 8 ? 8 : 16;
     p.ctas *= decode_ctas_per_sm(DP, rows <= 8 ? 1 : 2);
+    p.cuts = reinterpret_cast<int4*>(p.parts + 2ll * p.ctas * decode_slot(p.size));
     p.row_blocks = (rows + p.block_rows - 1) / p.block_rows;
     return rows <= 8 ? decode_keys<BF16, DP, 1>(p, stream) : decode_keys<BF16, DP, 2>(p, stream);
 }

@@ -50,6 +50,7 @@ struct DecodeParams {
     int ctas, least;
     float c;                                       // scale * log2(e)
     float* parts;                                  // slots of 16 x (size + 2) floats: sums, then maximum and sum of p per row
+    int4* cuts;                                    // for each CTA: what its end cuts (decode_cut)
     int* status;
 };
 
@@ -70,6 +71,11 @@ DLF_HD constexpr int decode_stages(int dp, int nb) { return dp <= 64 ? (nb == 1 
 DLF_HD constexpr int decode_stage_bytes(int dp) { return 16 * dp * 2 * 2; }  // a warp's 16 keys and values
 DLF_HD constexpr int decode_smem(int dp, int nb) { return kDecodeWarps * decode_stages(dp, nb) * decode_stage_bytes(dp); }
 DLF_HD constexpr int decode_slot(int size) { return 16 * (size + 2); }
+// A (sequence, head) that starts in a CTA's range and does not end there: sequence, head, slot of its first part, last CTA that
+// has a part of it (their slots are 2 c). No sequence: -1.
+__device__ __forceinline__ int4 decode_cut(const PlanWalk& w) {
+    return make_int4(w.b, w.head, w.slot(), (w.u + w.units - 1) / w.per);
+}
 
 template <bool BF16>
 DLF_HD constexpr float decode_lift() { return BF16 ? 0.0f : 7.0f; }  // p is taken times 2 to this
@@ -156,10 +162,12 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
     const int chunks = p.size / 8;
     const float c = p.c;
     bool bad_page = false;
+    int4 cut = make_int4(-1, 0, 0, 0);
 
     for (; walk.more(); walk.next()) {
         const int n_units = walk.count(), b = walk.b, len = walk.len, unit0 = walk.unit0;
         const bool whole = walk.whole();
+        if (unit0 == 0 && !whole) cut = decode_cut(walk);  // (the last segment)
         const int hk = walk.head / p.row_blocks, row0 = (walk.head - hk * p.row_blocks) * p.block_rows;
         const int rows = min(8 * NB, p.tokens * p.group - row0);
         // ---------------------------------------------------------------- copies
@@ -435,26 +443,23 @@ __global__ void __launch_bounds__(kDecodeThreads, decode_ctas_per_sm(DP, NB)) at
         }
         __syncthreads();  // before the rings are filled again
     }
+    if (threadIdx.x == 0) p.cuts[blockIdx.x] = cut;
     if (bad_page) atomicOr(p.status, DEV_STATUS_BAD_PAGE);
 }
 
-// Joins the partial results of a (sequence, kv head, row block): a block each. Those that one CTA had whole are done already.
+// Joins the partial results of the (sequence, kv head, row block) that the end of CTA blockIdx.x's range cuts first. The CTA left word
+// of it: looked up from the lengths by a block for each sequence and head, it took a batch's square (16384 sequences of 30 keys, 16
+// heads: 10.3 ms in all, 1.33 so).
 template <bool BF16>
 __global__ void __launch_bounds__(128) attention_join_kernel(const __grid_constant__ DecodeParams p) {
-    const int heads = p.kv_heads * p.row_blocks;
-    const int b = blockIdx.x / heads, hb = blockIdx.x - b * heads;
-    ptx::wait_for_dependencies();  // (before the lengths too: only behind it is what earlier kernels wrote visible)
-    int before, all;
-    plan_sums(decode_lengths(p), b, before, all);
-    const int per = plan_per(all * heads, p.ctas, p.least);
-    const int units = plan_units(plan_sequence(decode_lengths(p), b), kDecodeUnit);
-    const int first = before * heads + hb * units, last = first + units - 1;
-    const int c0 = first / per, c1 = last / per;
-    const int hk = hb / p.row_blocks, row0 = (hb - hk * p.row_blocks) * p.block_rows;
+    ptx::wait_for_dependencies();
+    const int4 cut = p.cuts[blockIdx.x];
+    const int b = cut.x, c0 = blockIdx.x, c1 = cut.w;
+    if (b < 0) return;
+    const int hk = cut.y / p.row_blocks, row0 = (cut.y - hk * p.row_blocks) * p.block_rows;
     const int rows = min(p.block_rows, p.tokens * p.group - row0), chunks = p.size / 4;
-    if (c0 == c1) return;
     const long long slot_floats = decode_slot(p.size);
-    const float* first_part = p.parts + plan_slot(first, per) * slot_floats;
+    const float* first_part = p.parts + cut.z * slot_floats;
     for (int id = threadIdx.x; id < rows * chunks; id += blockDim.x) {
         const int r = id / chunks, ch = id - r * chunks;
         // a running maximum, so that a part's statistics and values are asked for together

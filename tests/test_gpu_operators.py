@@ -559,6 +559,26 @@ def test_paged_attention_many_sequences():
     _check_paged(300, 90, 16, 2, 1, 64, torch.bfloat16)
 
 
+@pytest.mark.parametrize("b,longest,hk", [(3000, 40, 2), (1200, 700, 1), (20000, 64, 4), (5000, 65, 1)])
+def test_paged_attention_thousands_of_sequences(b, longest, hk):
+    """Sequences that a CTA has whole, and those that its end cuts, each once, empty ones among them."""
+    g = torch.Generator(device="cuda").manual_seed(b)
+    table, kp, vp = _cache(g, b, longest, 16, hk, 64, torch.float16)
+    lengths = torch.randint(0, longest + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+    q = torch.randn((b, 4, 64), generator=g, device="cuda").half()
+    y = torch.full_like(q, 7.0)
+    gdnn.paged_attention(q, kp, vp, table, lengths, y)
+    for i in range(0, b, 1000):
+        k, v = (t[table[i:i + 1000].long()].flatten(1, 2).double().repeat_interleave(4 // hk, 2) for t in (kp, vp))
+        keep = torch.arange(k.shape[1], device="cuda") < lengths[i:i + 1000, None]
+        s = (torch.einsum("bhd,bkhd->bhk", q[i:i + 1000].double(), k) / 8).masked_fill(~keep[:, None], -math.inf)
+        p = torch.softmax(s, -1).nan_to_num(0.0)
+        want, a = torch.einsum("bhk,bkhd->bhd", p, v), torch.einsum("bhk,bkhd->bhd", p, v.abs())
+        e = torch.einsum("bhd,bkhd->bhk", q[i:i + 1000].double().abs(), k.abs()).amax(-1, keepdim=True) / 8 * 66 * 2.0 ** -23
+        _check_rows(y[i:i + 1000], want, a, e, torch.float16, _half_step(torch.float16) ** 2)
+    assert dlf_b200.device_status() == 0
+
+
 @pytest.mark.parametrize("page", [6, 16])
 def test_pages_and_lengths_that_do_not_exist_are_left_out_and_reported(page):
     g = torch.Generator(device="cuda").manual_seed(page)
