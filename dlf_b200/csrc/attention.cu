@@ -61,11 +61,18 @@ bool strides_ok(std::initializer_list<size_t> s) {
     return true;
 }
 
+// A workspace may start anywhere; the parts in it, read and written in pieces of 16 bytes, start at the next multiple of 256.
+constexpr size_t kWorkspaceRoom = 256;
+float* workspace_parts(void* workspace) {
+    return reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(workspace) + kWorkspaceRoom - 1) / kWorkspaceRoom * kWorkspaceRoom);
+}
 // (sequences of one tile of keys are never cut)
-size_t tiles_workspace(size_t keys, size_t size) { return keys > kTileKeys ? static_cast<size_t>(2 * kB200Sms) * tiles_slot(static_cast<int>(size)) * 4 : 0; }
+size_t tiles_workspace(size_t keys, size_t size) {
+    return keys > kTileKeys ? static_cast<size_t>(2 * kB200Sms) * tiles_slot(static_cast<int>(size)) * 4 + kWorkspaceRoom : 0;
+}
 size_t decode_workspace(size_t size) {
     const size_t ctas = static_cast<size_t>(kB200Sms * decode_ctas_per_sm(static_cast<int>(size), 1));
-    return ctas * (2 * decode_slot(static_cast<int>(size)) * sizeof(float) + sizeof(int4));
+    return ctas * (2 * decode_slot(static_cast<int>(size)) * sizeof(float) + sizeof(int4)) + kWorkspaceRoom;
 }
 
 template <bool BF16, int DP, int KEYS, int NB, bool FULL>
@@ -236,7 +243,7 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
         p.ctas = std::min(dev.num_sms, kB200Sms);
         p.least = kDecodeLeast;
         p.c = c;
-        p.parts = static_cast<float*>(workspace);
+        p.parts = workspace_parts(workspace);
         p.status = dev.status;
         return decode_any(p, bf16, s);
     }
@@ -293,7 +300,7 @@ int dlf_b200_attention(const dlf_b200_attention_args* args, void* workspace, siz
     p.ctas = static_cast<int>(std::min<long long>(units, std::min(dev.num_sms, kB200Sms)));
     p.y = static_cast<char*>(y);
     p.y_sb = y_strides[0], p.y_st = y_strides[1], p.y_sh = y_strides[2];
-    p.parts = static_cast<float*>(workspace);
+    p.parts = workspace_parts(workspace);
     p.q_batched = q_strides[0] != 0;
     p.k_batched = k_strides[0] != 0;
     p.v_batched = v_strides[0] != 0;
@@ -366,7 +373,7 @@ int dlf_b200_paged_attention(const dlf_b200_paged_attention_args* args, void* wo
     p.ctas = std::min(dev.num_sms, kB200Sms);
     p.least = kDecodeLeast;
     p.c = scale * kLog2e;
-    p.parts = static_cast<float*>(workspace);
+    p.parts = workspace_parts(workspace);
     p.status = dev.status;
     return decode_any(p, dtype == DLF_B200_BFLOAT16, s);
 }

@@ -281,8 +281,8 @@ size_t dlf_b200_gemm_int8_workspace_bytes(size_t m, size_t n, size_t k, const si
  * dlf_b200_attention: Q and Y are (batch, queries, heads, size) with strides {batch, token, head}, K and V (batch, keys,
  * kv_heads, size) with theirs; a batch stride of 0 shares Q, K or V between the batch's entries. `key_lengths` (batch, device, or
  * NULL): keys of each entry that count, the rest is padding. `key_mask` (batch, keys, bytes; lines key_mask_ld apart, 0 = one line for
- * all; device, or NULL): 0 = the key does not count. `workspace`: dlf_b200_attention_workspace_bytes bytes of device memory (0 where none is
- * needed). Y must not overlap the inputs.
+ * all; device, or NULL): 0 = the key does not count. `workspace`: dlf_b200_attention_workspace_bytes bytes of device memory that start
+ * anywhere (0 where none is needed). Y must not overlap the inputs.
  *
  * dlf_b200_paged_attention: one query token for each sequence. Q and Y are (batch, heads, size) with strides {batch, head}; the
  * cache is (num_pages, page_size, kv_heads, size) with strides {page, token, head}; position i of sequence b lies in page

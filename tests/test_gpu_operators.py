@@ -832,6 +832,25 @@ def test_callers_scratch_is_used_and_too_little_is_refused():
     assert dlf_b200.device_status() == 0
 
 
+@pytest.mark.parametrize("start", [0, 1, 4, 8, 255])
+def test_callers_scratch_may_start_anywhere(start):
+    """With just what is needed, and nothing written beside it."""
+    calls = _calls(6)
+    L = dlf_b200.lib()
+    needs = [None, L.dlf_b200_attention_workspace_bytes(2, 1, 4000, 8, 2, 64), L.dlf_b200_attention_workspace_bytes(1, 200, 3000, 2, 1, 128),
+             L.dlf_b200_paged_attention_workspace_bytes(3, 4, 2, 64)]
+    needs[0] = needs[1]  # (the product asks for less)
+    for (f, out, want), need in zip(calls, needs):
+        own = torch.full((need + 512,), 77, dtype=torch.uint8, device="cuda")
+        at = (start - own.data_ptr()) % 256
+        out.zero_()
+        with gblas.scratch(own[at:at + need]):
+            f(None)
+        assert torch.equal(out, want)
+        assert bool((own[:at] == 77).all()) and bool((own[at + need:] == 77).all())
+    assert dlf_b200.device_status() == 0
+
+
 def test_results_do_not_depend_on_timing():
     calls = _calls(5)
     for _ in range(20):

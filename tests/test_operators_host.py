@@ -451,3 +451,13 @@ def test_kernels_read_no_device_memory_before_they_wait_for_the_kernel_before_th
         before, wait, _ = body.partition("wait_for_dependencies();")
         assert wait, body[:200]
         assert not re.search(r"plan_(sums|find|sequence)\(|PlanWalk walk|p\.(lengths|table|positions|sequences|mask|sa|sb)\[|\*reinterpret_cast<const", before), before[-400:]
+
+
+def test_workspaces_have_room_for_a_start_anywhere(built_lib):
+    """The parts of cut sequences (16 or 256 rows of size + 2 floats, two for each CTA) start on 16 bytes wherever the workspace does."""
+    L = built_lib
+    for size, ctas in ((8, 592), (64, 592), (72, 444), (128, 444)):
+        parts = ctas * (2 * 16 * (size + 2) * 4 + 16)
+        assert L.dlf_b200_paged_attention_workspace_bytes(3, 4, 2, size) >= parts + 15
+        assert L.dlf_b200_attention_workspace_bytes(3, 1, 600, 4, 2, size) >= parts + 15
+        assert L.dlf_b200_attention_workspace_bytes(3, 500, 600, 4, 2, size) >= 2 * 148 * 256 * (size + 2) * 4 + 15
