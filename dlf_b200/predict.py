@@ -722,7 +722,8 @@ class Predictor:
 
     ``int8`` runs the products with known weights (``Gemm`` / ``MatMul``, with the ``Relu`` that follows one) in 8-bit integers: a
     scale for each output channel of the weights and, found anew at every ``predict()``, for each row of the activations. The
-    results are those of weights and activations rounded to within half a 127th of their row's largest."""
+    results are those of weights and activations rounded, from the list's type, to within half a 127th of their row's largest.
+    The 8-bit weights take the place of the others on the device."""
 
     def __init__(self, graph, dtype=torch.float32, device=None, cuda_graph=True, channels_last=True, int8=False):
         if dtype not in _TORCH_TYPES:
@@ -833,6 +834,11 @@ class Predictor:
 
     # -- datums ---------------------------------------------------------------------------
 
+    def _upload(self, value):
+        """An initializer in the list's type on the device."""
+        return torch.from_numpy(np.ascontiguousarray(np.asarray(value.initializer, dtype=np.float64 if
+                                value.dtype == DataType.DOUBLE else np.float32))).to(self.dtype).to(self.device)
+
     def _alloc(self, value, like=None):
         """The device tensor of a value (OperatorFactory::alloc, predict.h:300-330): initializers
         are uploaded once, everything else is allocated once and reused by every ``predict()``."""
@@ -847,8 +853,7 @@ class Predictor:
                 if value.has_initializer():
                     t.copy_(_as_lengths(torch.from_numpy(np.ascontiguousarray(value.initializer))))
             elif value.has_initializer():
-                t = torch.from_numpy(np.ascontiguousarray(np.asarray(value.initializer, dtype=np.float64 if
-                                     value.dtype == DataType.DOUBLE else np.float32))).to(self.dtype).to(self.device)
+                t = self._upload(value)
             elif like is not None:
                 t = like.view(value.dims)
             elif id(value) in self._nhwc:
@@ -887,7 +892,10 @@ class Predictor:
             Y = self._alloc(n.output(0))
             return ConvOp(X, W, B, Y, _conv_filter(n, n.input(0).dims, n.input(1).dims), res, bool(n.get("relu")))
         if self._int8 and int8_product(n):
-            W = self._alloc(n.input(1))
+            # only the 8-bit weights stay: the others go when this operator is made, unless another one reads them
+            W = self._data.get(id(n.input(1)))
+            if W is None:
+                W = self._upload(n.input(1))
             if n.kind == "MatMul" or not n.get("transB", 0):
                 W = W.t().contiguous()
             bias = self._alloc(n.input(2))

@@ -461,3 +461,23 @@ def test_workspaces_have_room_for_a_start_anywhere(built_lib):
         assert L.dlf_b200_paged_attention_workspace_bytes(3, 4, 2, size) >= parts + 15
         assert L.dlf_b200_attention_workspace_bytes(3, 1, 600, 4, 2, size) >= parts + 15
         assert L.dlf_b200_attention_workspace_bytes(3, 500, 600, 4, 2, size) >= 2 * 148 * 256 * (size + 2) * 4 + 15
+
+
+def test_a_list_of_8_bit_products_keeps_no_other_weights(monkeypatch):
+    """But for those that an operator in floating point reads as well."""
+    _rounded_on_the_host(monkeypatch)
+    g = _gemm_relu_graph()
+    shared = g.addInitializer("w3", np.ones((3, 3), np.float32))
+    m = g.append("MatMul")
+    m.addInput(g.outputs.pop())
+    m.addInput(shared)
+    z = m.addOutput("u")
+    n = g.append("MatMul")  # weights times a value: in floating point
+    n.addInput(shared)
+    n.addInput(g.addInput("b", predict.DataType.FLOAT, (3, 2)))
+    for v in (z, n.addOutput("v")):
+        g.addOutput(v)
+    p = predict.Predictor(g, torch.float16, device="cpu", cuda_graph=False, int8=True)
+    assert [type(op).__name__ for op in p.operators] == ["Int8ProductOp"] * 3 + ["MatMulOp"]
+    weights = {id(v): v.name for v in g.inputs if v.has_initializer()}
+    assert [weights[i] for i in p._data if i in weights] == ["w3"]
