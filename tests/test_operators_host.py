@@ -481,3 +481,30 @@ def test_a_list_of_8_bit_products_keeps_no_other_weights(monkeypatch):
     assert [type(op).__name__ for op in p.operators] == ["Int8ProductOp"] * 3 + ["MatMulOp"]
     weights = {id(v): v.name for v in g.inputs if v.has_initializer()}
     assert [weights[i] for i in p._data if i in weights] == ["w3"]
+
+
+def test_results_allocated_for_another_stream_come_from_its_memory(built_lib, monkeypatch):
+    entered, allocated = [], []
+
+    class Stream:
+        def __init__(self, queue):
+            self.queue = queue
+
+        def __enter__(self):
+            entered.append(self.queue)
+
+        def __exit__(self, *exc):
+            entered.pop()
+
+    class Queue:
+        device_index, cuda_stream = 0, 0
+
+    empty, queue = torch.empty, Queue()
+    monkeypatch.setattr(torch.cuda, "stream", Stream)
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: (allocated.append(list(entered)), empty(*a, **kw))[1])
+    x, q, s = torch.zeros(4, 8), torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4)
+    for given, want in ((queue, [queue]), (None, [])):
+        allocated.clear()
+        _refused(StatusCode.kInvalidMatrixA, tensor.quantize, x, queue=given)  # (not on a device)
+        _refused(StatusCode.kInvalidMatrixA, tensor.matmul_int8, q, s, q, s, queue=given)
+        assert allocated == [want] * 3
