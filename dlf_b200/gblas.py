@@ -179,7 +179,8 @@ class _StreamScratch:
             stream = queue if queue is not None else torch.cuda.current_stream()
             if buf is not None:
                 buf.record_stream(stream)  # work queued earlier may still read the old buffer
-            buf = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+            with torch.cuda.stream(stream):  # (another stream's memory may still be in use by what is queued there)
+                buf = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
             buf.record_stream(stream)
             self.buffer = buf
         return buf

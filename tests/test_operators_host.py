@@ -508,3 +508,26 @@ def test_results_allocated_for_another_stream_come_from_its_memory(built_lib, mo
         _refused(StatusCode.kInvalidMatrixA, tensor.quantize, x, queue=given)  # (not on a device)
         _refused(StatusCode.kInvalidMatrixA, tensor.matmul_int8, q, s, q, s, queue=given)
         assert allocated == [want] * 3
+
+
+def test_a_streams_scratch_comes_from_its_memory(monkeypatch):
+    entered, allocated, queue = [], [], object()
+
+    class Stream:
+        def __init__(self, stream):
+            self.stream = stream
+
+        def __enter__(self):
+            entered.append(self.stream)
+
+        def __exit__(self, *exc):
+            entered.pop()
+
+    empty = torch.empty
+    monkeypatch.setattr(torch.cuda, "stream", Stream)
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: (allocated.append(list(entered)), empty(*a, **kw))[1])
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, stream: None)
+    scratch = gblas._StreamScratch()
+    for nbytes in (100, 50, 200):
+        assert scratch.at_least(nbytes, torch.device("cpu"), queue).numel() >= nbytes
+    assert allocated == [[queue]] * 2
