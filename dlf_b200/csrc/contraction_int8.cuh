@@ -135,9 +135,11 @@ __global__ void __launch_bounds__(kInt8Threads)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
     volatile int* abort_p = &abort_flag;
     const long long wait_limit = p.wait_limit;
-    // the weights on their way into L2 while the kernel before this one (the quantisation of the tokens) finishes
+    // The first of the weights, as many as the ring holds, on their way into L2 while the kernel before this one (the quantisation of the
+    // tokens) finishes. All of them would be more than L2 holds and get in the way of the loads themselves: 16 x 16384 x 16384 read
+    // 338 MB for 268 in 58.5 us, so 46.5 (none asked for: 48.2); 16 x 4096 x 4096 9.2 us either way (none: 9.7).
     if (CHANNELS && warp == 4 && ptx::elect_one())
-        for (int kb = kb0; kb < kb1; ++kb) ptx::tma_prefetch_3d(&tmL, kb * BK, l0, 0);
+        for (int kb = kb0; kb < min(kb1, kb0 + p.stages); ++kb) ptx::tma_prefetch_3d(&tmL, kb * BK, l0, 0);
     __syncwarp();
     ptx::wait_for_dependencies();
 
