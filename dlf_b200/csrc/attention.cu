@@ -160,7 +160,7 @@ int short_launch(ShortParams& p, int num_sms, const CUtensorMap& q, const CUtens
 }
 
 // Few queries: the kernel that runs through the keys for 16 rows (a token's heads of a group are rows too). It does as much work as
-// there are rows, the other one as if every head had 128 queries at least; with 32 entries of 1500 keys and 8 heads (us, this
+// there are rows, the other one as if every head had 128 queries at least; with 32 entries of 1500 keys and 8 heads, one to a kv head (us, this
 // kernel and the other): heads of 64 24 and 47 (16 queries), 33 and 47 (32), 53 and 48 (64); heads of 128 45 and 59 (16), 73 and
 // 60 (32). 32 query heads on one kv head, 1 query: 13 and 128.
 // Over up to 128 keys the other one is attention_short_kernel, and 8 queries are few: 256 entries of 77 keys, 8 heads (us), heads of

@@ -9,8 +9,8 @@
 // load, S, softmax, P V, store - that no unit fills, so what counts is how many tiles an SM has in flight, each at another place of its
 // chain: small blocks of four softmax warps (a thread a query row) and one warp for loads and products, four to an SM with heads of 64.
 //
-// Tensor memory: S in 128 columns, and in its place, when a chunk of 32 scores has been read for the second time, P (16-bit pairs,
-// the A operand of P V; chunk j goes to columns 16 j .., all of them read by then). With heads of 64 O lies in columns 64 .. 127, which P
+// Tensor memory: S in 128 columns, and in its place, when a chunk of 32 scores has been read for the second time, P (16-bit pairs, each p
+// rounded once as in attention_tiles.cuh, the A operand of P V; chunk j goes to columns 16 j .., all of them read by then). With heads of 64 O lies in columns 64 .. 127, which P
 // leaves free; with heads of 128 behind S. The scores are read twice (maximum; exponentials): a whole row does not fit into the
 // registers that four blocks leave.
 //

@@ -3,20 +3,25 @@
 //     S = Q K^T,  p = exp2(c (S - m)),  O = sum over key tiles of P V,  y = O / sum p      (c = scale * log2 e)
 //
 // The difference is taken first (attention_decode.cuh says why) where c m is beyond 2^10; below, the rounding of c m is 2^-14 at most,
-// and one fused step for c S - c m saves 3 % (2 x 4096 x 8192, 32 heads of 128: 758 us with the difference always, 735 so).
+// and one fused step for c S - c m saves 3 % (2 x 4096 x up to 8192, 32 heads of 128: 769 us with the difference always, 739 so).
 // m is a reference near the running maximum of a row: it is moved (and O and the sum scaled) only when the maximum has grown by
 // more than 2^8 since, which exp2's range allows and which makes the pass over O rare. In fp16 p is taken times 2^7, as in
 // attention_decode.cuh.
 //
-// Bound by power with heads of 128 values (2 x 4096 x 4096, 32 heads: 458 us, 1200 TFLOP/s, the clock at 1.6 GHz; every arrangement
-// below that was tried took the same time), by latencies and the special-function unit with heads of 64 (a pair of tiles of 128 x 128
-// scores costs the tensor core 1024 clocks and exp2, 16 a clock, 2048; it takes 3500).
+// With heads of 128 values (2 x 4096 x 4096, 32 heads: 506 us and 1090 TFLOP/s in a short run, 546 us and 1010 in a long one) the clock is
+// what gives way, 1.60 GHz at 990 W under the power cap; but no unit is full - tensor pipe 56 %, special-function unit 56 %, issue
+// slots 51 % - and plain products keep 1420 TFLOP/s under the same cap, so it is what this arrangement costs: S with both operands in
+// shared memory reads 8 KB in the 64 clocks of a product of 128 x 128 x 16, all that shared memory gives, and each tile of queries reads
+// K and V for itself. With heads of 64 latencies and the special-function unit (59 %; tensor pipe 29 %, the clock near its maximum): a
+// pair of tiles of 128 x 128 scores costs the tensor core 1024 clocks and exp2, 16 a clock, 2048; it takes 3500.
 //
 // Tensor memory (512 columns): O of the two tiles (DP columns each), P of the two tiles (16-bit pairs, 64 columns each; the A
 // operand of P V, so the scores never touch shared memory), and S: 128 columns for each tile with heads of 64, 128 columns that the tiles
 // use in turn with heads of 128. A thread takes its part of S into registers at once, so S is free again for the next product
 // while the exponentials are computed (with P in S's place the next S has to wait for P V). P is rounded to the 16-bit type
-// (the tensor core takes both operands of one type); O and the sums are 32-bit.
+// once (the tensor core takes both operands of one type, and a second part for the rest, as attention_decode.cuh has it, would be
+// half as many products again): an error of half a step of the type for each p, as large as that of the result's own rounding (bf16,
+// 4096 x 8192: 2.3e-3 in all, 1.7e-3 from the result's). O and the sums are 32-bit.
 //
 // Roles: warps 0-15 the softmax - 8 for each tile, a thread for half a query row (64 keys of a tile; the halves exchange their
 // maxima and sums through shared memory): with one thread a row (8 warps) heads of 64 and short rows took a tenth longer - 16 and

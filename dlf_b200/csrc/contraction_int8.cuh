@@ -341,7 +341,8 @@ __global__ void __launch_bounds__(kInt8Threads)
 // Persistent: pairs of CTAs walk through tiles of 256 x 256 (tokens x channels). Each CTA of a pair stages its 128 rows of A and
 // half the rows of B, one issuer drives both tensor cores (cta_group::2), which halves what B costs in shared-memory reads and
 // fills; the two accumulators of 256 columns take all of tensor memory, so a tile's epilogue runs beside the next
-// tile's products. Bound by the tensor core (and the power limit) from a depth of about 512 on, below by the epilogue's conversions.
+// tile's products. Bound by the tensor core (8192^3: 334 us in a short run) and, in a row, by the
+// power cap (381 us, 1.30 GHz at 993 W) from a depth of about 512 on, below by the epilogue's conversions.
 // Roles: warps 0-3 and 6-9 epilogue (quadrant = warp % 4, half of the columns each), 4 UMMA issuer and TMEM owner, 5 TMA producer.
 constexpr int kInt8PairThreads = 320;
 constexpr int kInt8PairStages = 6;
@@ -566,7 +567,8 @@ __global__ void __launch_bounds__(kInt8PairThreads, 1)
 }
 
 // Lines of an operand that start anywhere, copied so that they start on 16-byte boundaries (blockIdx.y: which operand); the bytes
-// past a line's end are zero. A thread writes 16 bytes from five aligned words (fewer at a line's ends).
+// past a line's end are zero. A thread writes 16 bytes from four aligned words; where the line starts off their boundaries from three and the
+// four bytes beside those one by one, so that nothing outside the line is read; the last bytes of a line one by one.
 struct Int8Lines {
     const signed char* src[2];
     signed char* dst[2];
@@ -592,8 +594,8 @@ __global__ void __launch_bounds__(256) int8_lines_kernel(const Int8Lines p) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) o[i] = reinterpret_cast<const uint32_t*>(at)[i];
             } else {
-                // the words that hold these 16 bytes lie between the line's own first and last bytes, but for the ends of the
-                // first and the last: those are read byte by byte
+                // three words lie between the first and the last of these 16 bytes; the two at the ends need not lie in the line: what
+                // is wanted of them is read byte by byte
                 uint32_t w[5];
                 const uint32_t* a = reinterpret_cast<const uint32_t*>(at - off);
                 w[0] = 0u;

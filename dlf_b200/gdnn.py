@@ -411,7 +411,9 @@ def attention(Q, K, V, Y, scale=None, key_lengths=None, key_mask=None, queue=Non
     128, heads a multiple of kv_heads (head h reads kv head h // (heads // kv_heads)); ``scale`` is 1 / sqrt(size) if not given.
 
     ``key_lengths`` (batch, int32) and ``key_mask`` (batch, keys; bool or uint8, 0 = left out) say which keys count; those that do not
-    may hold anything. A query with no key gets zeros. Any strides that are multiples of 8 elements, over 16-byte aligned
+    may hold anything. A query with no key gets zeros. Scores, their statistics and all sums have 32 bits; a key's weight is rounded to the
+    values' type once where there are many queries, and kept in two parts where there are few (up to 32 with heads of up to 64 values, else 16;
+    over up to 128 keys 8). Any strides that are multiples of 8 elements, over 16-byte aligned
     addresses, with a head's values contiguous; Q, K, V and the mask may be shared by the batch (expanded). Y must not overlap the
     inputs."""
     if scale is not None:
@@ -488,8 +490,8 @@ def _append_plan(K, V, K_pages, V_pages, page_table):
 
 def paged_append(K, V, K_pages, V_pages, page_table, positions, sequences=None, queue=None, event=None):
     """New keys and values K and V (tokens, kv_heads, size) into a paged cache (see ``paged_attention``): token i to position
-    positions[i] of sequence sequences[i] (both int32; without ``sequences``, of sequence i). A position below 0 marks a token that is padding and goes nowhere. The rest
-    of the cache stays as it is."""
+    positions[i] of sequence sequences[i] (both int32; without ``sequences``, of sequence i). A position below 0 marks a token that is padding and goes
+    nowhere. The rest of the cache stays as it is."""
     key = (K.dtype, V.dtype, K_pages.dtype, V_pages.dtype, page_table.dtype, K.device, V.device, K_pages.device, V_pages.device,
            page_table.device, K.shape, V.shape, K_pages.shape, V_pages.shape, page_table.shape, K.stride(), V.stride(), K_pages.stride(),
            V_pages.stride(), page_table.stride())

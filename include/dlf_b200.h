@@ -272,11 +272,14 @@ size_t dlf_b200_gemm_int8_workspace_bytes(size_t m, size_t n, size_t k, const si
 
 /* Attention of the queries of a decoder (or of an image) over an encoder's states, or of one new token over a paged cache:
  *     Y = softmax(scale * Q K^T over the kept keys) V                    for each head
- * with 32-bit scores, softmax statistics and sums. Types: Half and BFloat16 (else kNotImplemented). `heads` query heads share
+ * with 32-bit scores, softmax statistics and sums. The weight of a key meets its values rounded to their 16-bit type, in two parts (the
+ * rounding and the rest) where the queries are few - up to 32 with heads of up to 64 values, else 16, over up to 128 keys 8 - and once, an
+ * error of half a step of that type, where they are more. Types: Half and BFloat16 (else kNotImplemented). `heads` query heads share
  * `kv_heads` heads of keys and values (heads a multiple of kv_heads; head h reads kv head h / (heads / kv_heads)). A head's
  * `size` values are contiguous: a multiple of 8 up to 128. The other strides are counted in elements and arbitrary, but multiples
- * of 8 over 16-byte aligned bases (kNotImplemented else). scale > 0. A row of which no key is kept is zeros. What is
- * masked out is not used, whatever it is (infinities, NaN). Nothing is kept between calls.
+ * of 8 over 16-byte aligned bases (kNotImplemented else). scale > 0. A row of which no key is kept, or whose scores are
+ * all -infinity, is zeros. What is masked out is not used, whatever it is (infinities, NaN); a score that counts and is NaN or +infinity makes
+ * its row NaN, an infinite value that counts makes its row infinite or NaN. Nothing is kept between calls.
  *
  * dlf_b200_attention: Q and Y are (batch, queries, heads, size) with strides {batch, token, head}, K and V (batch, keys,
  * kv_heads, size) with theirs; a batch stride of 0 shares Q, K or V between the batch's entries. `key_lengths` (batch, device, or
