@@ -14,7 +14,10 @@
 // leaves free; with heads of 128 behind S. The scores are read twice (maximum; exponentials): a whole row does not fit into the
 // registers that four blocks leave.
 //
-// 16 x 4096 queries over 77 keys, 8 heads: 33 us with heads of 64, 54 with heads of 128 (21 and 42 at the copy rate); attention_tiles.cuh,
+// The difference is always taken first: the choice that attention_tiles.cuh makes by the size of c m costs more here than it saves (16 x
+// 4096 queries over 128 keys, 8 heads of 64: 42.7 us with it, 41.8 without).
+//
+// 16 x 4096 queries over 77 keys, 8 heads: 34 us with heads of 64, 54 with heads of 128 (21 and 42 at the copy rate); attention_tiles.cuh,
 // whose block has two tiles in flight that its barriers keep in step, takes 46 and 89.
 //
 // A block runs through consecutive tiles of queries, so the keys and values of a kv head are loaded once for all of a block's tiles of
