@@ -179,8 +179,7 @@ class _StreamScratch:
             stream = queue if queue is not None else torch.cuda.current_stream()
             if buf is not None:
                 buf.record_stream(stream)  # work queued earlier may still read the old buffer
-            with torch.cuda.stream(stream):  # (another stream's memory may still be in use by what is queued there)
-                buf = torch.empty(int(nbytes), dtype=torch.uint8, device=device)
+            buf = _empty(int(nbytes), torch.uint8, device, stream)
             buf.record_stream(stream)
             self.buffer = buf
         return buf
@@ -190,6 +189,13 @@ def _stream_scratch(table, device, handle):
     key = (device.index, handle)
     entry = table.get(key)
     return entry if entry is not None else table.setdefault(key, _StreamScratch())
+
+
+def _empty(shape, dtype, device, queue):
+    """Memory that a call on `queue` (None = the current stream) writes: that stream's, as another one's may still be in use by what is
+    queued there."""
+    with torch.cuda.stream(queue) if queue is not None else _NO_LOCK:
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 _KEPT_BYTES = 64 << 20  # of a product's scratch: the partial sums of a K-split fit, copies of large operands do not
@@ -511,10 +517,7 @@ def gemmBatched(layout, a_transpose, b_transpose, m, n, k, alphas, a_buffer, a_o
     need = lib().dlf_b200_gemm_batched_workspace_bytes(batch_count)
     s, sp = _stream(queue)
     if workspace is None:
-        workspace = torch.empty(max(need, 8), dtype=torch.uint8, device=c_buffer.device)
-        # the tables are read by work queued on `s`, which may not be the allocator's current
-        # stream: the block must not be handed out again before that work has passed
-        workspace.record_stream(s)
+        workspace = _empty(max(need, 8), torch.uint8, c_buffer.device, queue)
     arr = ctypes.c_size_t * batch_count
     ao, bo, co = arr(*map(int, a_offsets)), arr(*map(int, b_offsets)), arr(*map(int, c_offsets))
     al_keep, al = _scalars(alphas, c_buffer.dtype)
@@ -552,11 +555,9 @@ class Side(enum.IntEnum):
 _SYMM, _SYRK, _TRMM, _TRSM = 1, 2, 3, 4
 
 
-def _level3_workspace(routine, buf, m, n, stream):
+def _level3_workspace(routine, buf, m, n, queue):
     need = lib().dlf_b200_level3_workspace_bytes(routine, int(precision_of(buf)), m, n)
-    ws = torch.empty(max(int(need), 8), dtype=torch.uint8, device=buf.device)
-    ws.record_stream(stream)  # read by work queued on `stream`, which may not be the allocator's
-    return ws
+    return _empty(max(int(need), 8), torch.uint8, buf.device, queue)
 
 
 def symm(layout, side, triangle, m, n, alpha, a_buffer, a_offset, a_ld, b_buffer, b_offset, b_ld, beta,
@@ -576,7 +577,7 @@ def symm(layout, side, triangle, m, n, alpha, a_buffer, a_offset, a_ld, b_buffer
     _test_matrix(one, two, c_buffer, c_offset, c_ld, StatusCode.kInvalidLeadDimC, StatusCode.kInsufficientMemoryC)
     al, be = _scalar(alpha, c_buffer.dtype), _scalar(beta, c_buffer.dtype)
     s, sp = _stream(queue)
-    ws = _level3_workspace(_SYMM, c_buffer, m, n, s)
+    ws = _level3_workspace(_SYMM, c_buffer, m, n, queue)
     if event is not None:
         event.start.record(s)
     rc = lib().dlf_b200_symm(int(prec), int(layout), int(side), int(triangle), m, n, ctypes.byref(al),
@@ -602,7 +603,7 @@ def syrk(layout, triangle, a_transpose, n, k, alpha, a_buffer, a_offset, a_ld, b
     _test_matrix(n, n, c_buffer, c_offset, c_ld, StatusCode.kInvalidLeadDimC, StatusCode.kInsufficientMemoryC)
     al, be = _scalar(alpha, c_buffer.dtype), _scalar(beta, c_buffer.dtype)
     s, sp = _stream(queue)
-    ws = _level3_workspace(_SYRK, c_buffer, n, n, s)
+    ws = _level3_workspace(_SYRK, c_buffer, n, n, queue)
     if event is not None:
         event.start.record(s)
     rc = lib().dlf_b200_syrk(int(prec), int(layout), int(triangle), int(a_transpose), n, k, ctypes.byref(al),
@@ -633,9 +634,7 @@ def _triangular(fn_name, routine, layout, side, triangle, a_transpose, diagonal,
     need = L.dlf_b200_level3_workspace_bytes(routine, int(prec), m, n)
     ws = None
     if need:
-        ws = torch.empty(int(need), dtype=torch.uint8, device=b.device)
-        if queue is not None:
-            ws.record_stream(queue)  # read by work queued on a stream that may not be the allocator's
+        ws = _empty(int(need), torch.uint8, b.device, queue)
     if event is not None:
         s = queue if queue is not None else torch.cuda.current_stream()
         event.start.record(s)

@@ -13,7 +13,7 @@ import struct
 import torch
 
 from . import lib
-from .gblas import (BLASError, StatusCode, _NO_LOCK, _Plans, _caller_scratch, _capturing, _check, _operator_scratch,
+from .gblas import (BLASError, StatusCode, _NO_LOCK, _Plans, _caller_scratch, _capturing, _check, _empty, _operator_scratch,
                     _operator_stream, _passing_scratch, _ptr, _stream, _stream_scratch, precision_of)
 
 
@@ -252,9 +252,11 @@ def pack_filters_nhwc(W, queue=None):
     prec = precision_of(W)
     co, c, kh, kw = (int(d) for d in W.shape)
     n = lib().dlf_b200_nhwc_filter_elems(c, co, kh, kw)
-    out = torch.empty(n, dtype=W.dtype, device=W.device)
+    with torch.cuda.stream(queue) if queue is not None else _NO_LOCK:
+        W = W.contiguous()
+    out = _empty(n, W.dtype, W.device, queue)
     _, sp = _stream(queue)
-    _check(lib().dlf_b200_pack_filters_nhwc(int(prec), c, co, kh, kw, _ptr(W.contiguous()), _ptr(out), sp))
+    _check(lib().dlf_b200_pack_filters_nhwc(int(prec), c, co, kh, kw, _ptr(W), _ptr(out), sp))
     return out
 
 
@@ -264,7 +266,7 @@ def nchw_to_nhwc(X, Y=None, queue=None):
     n, c, h, w = (int(d) for d in X.shape)
     cp = (c + 7) // 8 * 8
     if Y is None:
-        Y = torch.empty((n, h, w, cp), dtype=X.dtype, device=X.device)
+        Y = _empty((n, h, w, cp), X.dtype, X.device, queue)
     elif Y.numel() < n * h * w * cp or Y.dtype != X.dtype:
         raise BLASError(StatusCode.kInsufficientMemoryC)
     _, sp = _stream(queue)

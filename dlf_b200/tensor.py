@@ -253,12 +253,6 @@ def matmul(A, B, C=None, alpha=1, beta=0, backend=None, trace=None):
     return C
 
 
-def _empty(shape, dtype, device, queue):
-    """A result that a call on ``queue`` writes: from that stream's memory (another stream's may still be in use by what is queued there)."""
-    with torch.cuda.stream(queue) if queue is not None else _gblas._NO_LOCK:
-        return torch.empty(shape, dtype=dtype, device=device)
-
-
 _QUANTIZE_PLANS, _INT8_PLANS = _gblas._Plans(), _gblas._Plans()
 
 
@@ -305,9 +299,9 @@ def quantize(X, Q=None, scales=None, queue=None, event=None):
         raise ShapeError("quantize: X must have rows")
     if Q is None:
         n = X.shape[-1]
-        Q = _empty(X.shape[:-1] + ((n + 15) // 16 * 16,), torch.int8, X.device, queue)[..., :n]
+        Q = _gblas._empty(X.shape[:-1] + ((n + 15) // 16 * 16,), torch.int8, X.device, queue)[..., :n]
     if scales is None:
-        scales = _empty(X.shape[:-1], torch.float32, X.device, queue)
+        scales = _gblas._empty(X.shape[:-1], torch.float32, X.device, queue)
     key = (X.dtype, Q.dtype, scales.dtype, X.device, Q.device, scales.device, X.shape, Q.shape, scales.shape, X.stride(), Q.stride(),
            scales.stride())
     plan = _QUANTIZE_PLANS.get(key)
@@ -345,7 +339,7 @@ def matmul_int8(A, a_scales, B, b_scales, C=None, bias=None, activation=None, dt
     with one for each of its rows (output channel): a quantised layer (``gblas.gemmInt8``). C (..., n) is allocated with
     ``dtype`` when not given. Rows of A and B that lie on 16-byte boundaries are read as they are, others are copied first."""
     if C is None:
-        C = _empty(A.shape[:-1] + B.shape[:1], dtype, A.device, queue)
+        C = _gblas._empty(A.shape[:-1] + B.shape[:1], dtype, A.device, queue)
     key = (A.dtype, B.dtype, C.dtype, a_scales.dtype, b_scales.dtype, A.device, B.device, C.device, a_scales.device, b_scales.device, A.shape,
            B.shape, C.shape, a_scales.shape, b_scales.shape, A.stride(), B.stride(), C.stride(), a_scales.stride(), b_scales.stride(), activation,
            None if bias is None else (bias.dtype, bias.device, bias.shape, bias.stride()))

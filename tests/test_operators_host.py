@@ -531,3 +531,41 @@ def test_a_streams_scratch_comes_from_its_memory(monkeypatch):
     for nbytes in (100, 50, 200):
         assert scratch.at_least(nbytes, torch.device("cpu"), queue).numel() >= nbytes
     assert allocated == [[queue]] * 2
+
+
+def test_other_calls_on_another_stream_take_that_streams_memory(monkeypatch):
+    """Packed filters, channels-last copies, the tables and the scratch of batched products and of level 3."""
+    entered, allocated = [], []
+
+    class Stream:
+        def __init__(self, queue):
+            self.queue = queue
+
+        def __enter__(self):
+            entered.append(self.queue)
+
+        def __exit__(self, *exc):
+            entered.pop()
+
+    class Queue:
+        device_index, cuda_stream = 0, 0
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: 64 if name.endswith(("_bytes", "_elems")) else 0
+
+    empty, queue = torch.empty, Queue()
+    monkeypatch.setattr(torch.cuda, "stream", Stream)
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: (allocated.append(list(entered)), empty(*a, **kw))[1])
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda self, stream: None)
+    for module in (gblas, gdnn):
+        monkeypatch.setattr(module, "lib", Library)
+        monkeypatch.setattr(module, "_ptr", lambda buf, offset=0: buf.data_ptr())
+    x = torch.zeros(1, 8, 4, 4)
+    gdnn.pack_filters_nhwc(x, queue=queue)
+    gdnn.nchw_to_nhwc(x, queue=queue)
+    m = torch.zeros(16)
+    gblas.gemmBatched(gblas.Layout.RowMajor, gblas.Transpose.NoTrans, gblas.Transpose.NoTrans, 4, 4, 4, [1.0], m, [0], 4, m, [0], 4, [0.0], m, [0], 4, 1,
+                      queue=queue)
+    gblas.symm(gblas.Layout.RowMajor, gblas.Side.Left, gblas.Triangle.Upper, 4, 4, 1.0, m, 0, 4, m, 0, 4, 0.0, m, 0, 4, queue=queue)
+    assert allocated == [[queue]] * 4
